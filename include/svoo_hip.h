@@ -278,6 +278,59 @@ int svoo_exact_sparsity_counts(const uint16_t* scores, long long rows, int n, fl
                                int32_t* counts, void* stream);
 
 /* ---------------------------------------------------------------------------------------------
+ * Layer norm over rows of `cols` elements (1..16384), x [batch][rows_per_batch][cols] with strides in elements and
+ * contiguous columns, any address.  n = (x - mean) rstd, rstd = 1 / sqrt(var + eps), statistics in fp32;
+ *   y = n w + b, or with `modulated` y = n (1 + w) + b.  w and b ([cols] per batch entry, 0 as the batch stride for shared
+ *   ones, NULL for none) and every other tensor have an element type: 0 bf16, 1 fp16, 2 fp32.
+ *   svoo_layer_norm_fwd: y [batch * rows_per_batch][cols], or instead 8-bit rows q and q_scale as svoo_fp8_quantize_rows
+ *     makes them (fp8_type) of the y that y_type would hold; mean and rstd (fp32, one per row) are optional.
+ *   svoo_layer_norm_bwd: dx (type of x, contiguous), dw and db ([batch][cols]; pass batch 1 for shared parameters), each
+ *     optional.  The sums over rows are fp32 in a fixed order.
+ * Beside the norms and modulation of svoo/models/wan/custom_models.py:23-109.
+ * ------------------------------------------------------------------------------------------- */
+int svoo_layer_norm_fwd(const void* x, int x_type, long long x_batch_stride, long long x_row_stride, const void* w,
+                        int w_type, long long w_batch_stride, const void* b, int b_type, long long b_batch_stride,
+                        int modulated, float eps, long long batch, long long rows_per_batch, int cols, void* y,
+                        int y_type, uint8_t* q, uint8_t* q_scale, int fp8_type, float* mean, float* rstd, void* stream);
+size_t svoo_layer_norm_bwd_workspace_size(long long batch, long long rows_per_batch, int cols);
+int svoo_layer_norm_bwd(const void* x, int x_type, long long x_batch_stride, long long x_row_stride, const void* dy,
+                        int dy_type, long long dy_batch_stride, long long dy_row_stride, const void* w, int w_type,
+                        long long w_batch_stride, int modulated, const float* mean, const float* rstd, long long batch,
+                        long long rows_per_batch, int cols, void* dx, void* dw, int dw_type, void* db, int db_type,
+                        void* workspace, size_t ws_bytes, void* stream);
+
+/* ---------------------------------------------------------------------------------------------
+ * 8-bit matrices with a power-of-two scale per block of 128 (no reference counterpart).  Types: 0 e4m3, 1 e5m2 (OCP).
+ * A block's scale is 2^e, e the smallest with amax 2^-e within the type's range (448, 57344) over its finite values, not
+ * below -127, 0 for an all-zero block, stored as the byte e + 127 (e8m0).  Values are rounded to nearest even; NaN stays,
+ * infinities become NaN in e4m3.  Rows of values are padded with zeros to whole blocks: for `cols` columns a row takes
+ * 128 ceil(cols / 128) bytes and ceil(cols / 128) scales, both contiguous from row to row.
+ *   svoo_fp8_quantize_rows: blocks of 128 columns of one row.
+ *   svoo_fp8_quantize_tiles: with `square` blocks of 128 x 128 (q [rows][..], scale [ceil(rows/128)][ceil(cols/128)], and /
+ *     or the transposes qt [cols][..], scale_t); otherwise rows as above in q and the transposed matrix, in blocks of
+ *     128 of ITS columns, in qt and scale_t, and optionally the column sums of x (not with `square`; needs the workspace).
+ *   svoo_fp8_dequantize: the values q 2^e, rounded to `type`.
+ *   svoo_fp8_matmul: c[m][n] = act(sum_k a[m][k] b[n][k] + bias[n]) of the matrices that (a, a_scale) and (b, b_scale) stand
+ *     for, accumulated in fp32 and rounded once; k counts the padded columns; b is e4m3 with a scale per row or per 128
+ *     rows; row strides in bytes, rows at 16-byte addresses; act 0 none, 1 GELU (tanh form).
+ * ------------------------------------------------------------------------------------------- */
+int svoo_fp8_quantize_rows(const void* x, int type, long long x_row_stride, long long rows, long long cols, int fp8_type,
+                           uint8_t* q, uint8_t* scale, void* stream);
+size_t svoo_fp8_quantize_tiles_workspace_size(long long rows, long long cols);
+int svoo_fp8_quantize_tiles(const void* x, int type, long long x_row_stride, long long rows, long long cols, int fp8_type,
+                            int square, uint8_t* q, uint8_t* scale, uint8_t* qt, uint8_t* scale_t, void* col_sums,
+                            int col_sums_type, void* workspace, size_t ws_bytes, void* stream);
+int svoo_fp8_dequantize(const uint8_t* q, long long q_row_stride, const uint8_t* scale, long long scale_row_stride,
+                        int rows_per_scale, long long rows, long long cols, int fp8_type, void* y, int type,
+                        void* stream);
+size_t svoo_fp8_matmul_workspace_size(long long m, long long n, long long k);
+int svoo_fp8_matmul(const uint8_t* a, long long a_row_stride, const uint8_t* a_scale, long long a_scale_row_stride,
+                    int a_type, const uint8_t* b, long long b_row_stride, const uint8_t* b_scale,
+                    long long b_scale_row_stride, int b_rows_per_scale, const void* bias, int bias_type, int act,
+                    long long m, long long n, long long k, void* c, int c_type, void* workspace, size_t ws_bytes,
+                    void* stream);
+
+/* ---------------------------------------------------------------------------------------------
  * Diagnostic (no reference counterpart): runs one v_mfma_f32_32x32x16_bf16 and one
  * v_mfma_f32_16x16x32_bf16 on index-coded operands and writes the raw per-lane accumulators
  * (out32: 64 lanes x 16 floats, out16: 64 lanes x 4 floats), so tests can confirm the operand

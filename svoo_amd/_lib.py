@@ -56,6 +56,20 @@ _SIGS = {
     "svoo_ear_select": (c_int, [P, P, P, P, P, P, c_int, c_int, c_int, c_int, c_float, P, P]),
     "svoo_qkv_heads": (c_int, [P, P, P, c_longlong, c_longlong, c_longlong, P, P, P, c_int, c_int, c_int, c_int, c_int,
                                c_int, P, P, c_float, c_float, P, P, c_int, c_int, P]),
+    "svoo_layer_norm_fwd": (c_int, [P, c_int, c_longlong, c_longlong, P, c_int, c_longlong, P, c_int, c_longlong, c_int,
+                                    c_float, c_longlong, c_longlong, c_int, P, c_int, P, P, c_int, P, P, P]),
+    "svoo_layer_norm_bwd_workspace_size": (c_size_t, [c_longlong, c_longlong, c_int]),
+    "svoo_layer_norm_bwd": (c_int, [P, c_int, c_longlong, c_longlong, P, c_int, c_longlong, c_longlong, P, c_int,
+                                    c_longlong, c_int, P, P, c_longlong, c_longlong, c_int, P, P, c_int, P, c_int, P,
+                                    c_size_t, P]),
+    "svoo_fp8_quantize_rows": (c_int, [P, c_int, c_longlong, c_longlong, c_longlong, c_int, P, P, P]),
+    "svoo_fp8_quantize_tiles_workspace_size": (c_size_t, [c_longlong, c_longlong]),
+    "svoo_fp8_quantize_tiles": (c_int, [P, c_int, c_longlong, c_longlong, c_longlong, c_int, c_int, P, P, P, P, P, c_int,
+                                        P, c_size_t, P]),
+    "svoo_fp8_dequantize": (c_int, [P, c_longlong, P, c_longlong, c_int, c_longlong, c_longlong, c_int, P, c_int, P]),
+    "svoo_fp8_matmul_workspace_size": (c_size_t, [c_longlong, c_longlong, c_longlong]),
+    "svoo_fp8_matmul": (c_int, [P, c_longlong, P, c_longlong, c_int, P, c_longlong, P, c_longlong, c_int, P, c_int, c_int,
+                                c_longlong, c_longlong, c_longlong, P, c_int, P, c_size_t, P]),
     "svoo_vbsa_ear_fwd": (c_int, [P, P, P, P, P, P, P, P, P, c_int, c_int, c_int, c_int, c_int, P, c_size_t, P, P]),
 }
 
@@ -94,6 +108,16 @@ def call(name: str, *args) -> None:
         raise RuntimeError(f"{name} failed ({rc}): {last_error()}")
 
 
+def launch(device: torch.device, name: str, *args) -> None:
+    """:func:`call` with the current stream of ``device`` as the last argument, on that device (a launch goes to the
+    current one)."""
+    if device.index == torch.cuda.current_device():
+        call(name, *args, stream_of(device))
+    else:
+        with torch.cuda.device(device):
+            call(name, *args, stream_of(device))
+
+
 def ptr(t: Optional[torch.Tensor]) -> Optional[int]:
     """Device pointer of a tensor (None -> NULL)."""
     if t is None:
@@ -126,6 +150,21 @@ def convert(x: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
     call("svoo_convert", xx.data_ptr(), _ELEM_TYPES[xx.dtype], out.data_ptr(), _ELEM_TYPES[dtype], xx.numel(),
          stream_of(xx.device))
     return out
+
+
+def elem_type(t: torch.Tensor, name: str) -> int:
+    """The C ABI's code of a tensor's element type (bf16, fp16 or fp32), on the GPU."""
+    if not isinstance(t, torch.Tensor) or t.dtype not in _ELEM_TYPES:
+        raise TypeError(f"{name}: the MI355X path takes bfloat16, float16 or float32 tensors, got "
+                        f"{getattr(t, 'dtype', type(t).__name__)}")
+    require_gpu_tensor(t, name)
+    return _ELEM_TYPES[t.dtype]
+
+
+def refuse_grad(name: str, *tensors) -> None:
+    """An operator without a backward pass takes no tensor that waits for a gradient: its result would end the graph."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise RuntimeError(f"{name} has no backward pass: call it under torch.no_grad() or on detached tensors")
 
 
 def as_bf16(x: torch.Tensor, name: str) -> torch.Tensor:

@@ -1,0 +1,173 @@
+// Eight consecutive elements of a row per lane, whatever the element type and the row's address; sums and maxima over
+// the lanes of a row; 8-bit values with a power-of-two scale per block of 128.
+#pragma once
+
+#include "svoo_common.h"
+
+namespace svoo {
+
+enum RowType { kRowBf16 = 0, kRowF16 = 1, kRowF32 = 2 };
+enum Fp8Type { kFp8E4m3 = 0, kFp8E5m2 = 1 };
+
+// Four dwords at any byte address (gfx950's global loads and stores need no alignment).
+struct __attribute__((packed, aligned(1))) Dwords4 { u32x4_t v; };
+struct __attribute__((packed, aligned(1))) Dwords2 { uint32_t v[2]; };
+
+__device__ __forceinline__ float row_elem(const void* p, int type, long long i) {
+  if (type == kRowBf16) return bf16_to_f32(((const uint16_t*)p)[i]);
+  if (type == kRowF16) return (float)__builtin_bit_cast(_Float16, ((const uint16_t*)p)[i]);
+  return ((const float*)p)[i];
+}
+
+__device__ __forceinline__ void set_row_elem(void* p, int type, long long i, float v) {
+  if (type == kRowBf16) ((uint16_t*)p)[i] = f32_to_bf16(v);
+  else if (type == kRowF16) ((uint16_t*)p)[i] = __builtin_bit_cast(uint16_t, (_Float16)v);
+  else ((float*)p)[i] = v;
+}
+
+// v as the row's type holds it.
+__device__ __forceinline__ float row_round(int type, float v) {
+  if (type == kRowBf16) return bf16_round_f32(v);
+  if (type == kRowF16) return (float)(_Float16)v;
+  return v;
+}
+
+// Elements i .. i + 7 of a row, the first n of them (n <= 0: none) and zeros.  kWhole: n is a multiple of 8.
+template <int T, bool kWhole = false>
+__device__ __forceinline__ void load_row8(const void* p, long long i, int n, float (&f)[8]) {
+  if (n >= 8) {
+    if (T == kRowF32) {
+      const u32x4_t a = ((const Dwords4*)((const float*)p + i))->v, b = ((const Dwords4*)((const float*)p + i + 4))->v;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        f[e] = __uint_as_float(a[e]);
+        f[4 + e] = __uint_as_float(b[e]);
+      }
+    } else {
+      const u32x4_t w = ((const Dwords4*)((const uint16_t*)p + i))->v;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const uint16_t b = (uint16_t)(w[e / 2] >> (16 * (e & 1)));
+        f[e] = T == kRowBf16 ? bf16_to_f32(b) : (float)__builtin_bit_cast(_Float16, b);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] = !kWhole && e < n ? row_elem(p, T, i + e) : 0.0f;
+  }
+}
+
+template <int T, bool kWhole = false>
+__device__ __forceinline__ void store_row8(void* p, long long i, int n, const float (&f)[8]) {
+  if (n >= 8) {
+    if (T == kRowF32) {
+      ((Dwords4*)((float*)p + i))->v = u32x4_t{__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]),
+                                               __float_as_uint(f[3])};
+      ((Dwords4*)((float*)p + i + 4))->v = u32x4_t{__float_as_uint(f[4]), __float_as_uint(f[5]), __float_as_uint(f[6]),
+                                                   __float_as_uint(f[7])};
+    } else {
+      u32x4_t w;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if (T == kRowBf16) {
+          w[e] = cvt_pk_bf16(f[2 * e], f[2 * e + 1]);
+        } else {
+          w[e] = (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)f[2 * e]) |
+                 ((uint32_t)__builtin_bit_cast(uint16_t, (_Float16)f[2 * e + 1]) << 16);
+        }
+      }
+      ((Dwords4*)((uint16_t*)p + i))->v = w;
+    }
+  } else if (!kWhole) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (e < n) set_row_elem(p, T, i + e, f[e]);
+  }
+}
+
+// A row's share of lane t of TPR: NC chunks of eight elements, (c TPR + t) 8 .. + 7 of cols.  The type is uniform, so its
+// branch is outside the loop and a row's loads leave together.
+template <int TPR, int NC, bool kWhole>
+__device__ __forceinline__ void load_row(const void* p, int type, long long at, int cols, int t, float (&v)[NC][8]) {
+  if (type == kRowBf16) {
+#pragma unroll
+    for (int c = 0; c < NC; ++c) load_row8<kRowBf16, kWhole>(p, at + (c * TPR + t) * 8, cols - (c * TPR + t) * 8, v[c]);
+  } else if (type == kRowF16) {
+#pragma unroll
+    for (int c = 0; c < NC; ++c) load_row8<kRowF16, kWhole>(p, at + (c * TPR + t) * 8, cols - (c * TPR + t) * 8, v[c]);
+  } else {
+#pragma unroll
+    for (int c = 0; c < NC; ++c) load_row8<kRowF32, kWhole>(p, at + (c * TPR + t) * 8, cols - (c * TPR + t) * 8, v[c]);
+  }
+}
+template <int TPR, int NC, bool kWhole>
+__device__ __forceinline__ void store_row(void* p, int type, long long at, int cols, int t, const float (&v)[NC][8]) {
+  if (type == kRowBf16) {
+#pragma unroll
+    for (int c = 0; c < NC; ++c) store_row8<kRowBf16, kWhole>(p, at + (c * TPR + t) * 8, cols - (c * TPR + t) * 8, v[c]);
+  } else if (type == kRowF16) {
+#pragma unroll
+    for (int c = 0; c < NC; ++c) store_row8<kRowF16, kWhole>(p, at + (c * TPR + t) * 8, cols - (c * TPR + t) * 8, v[c]);
+  } else {
+#pragma unroll
+    for (int c = 0; c < NC; ++c) store_row8<kRowF32, kWhole>(p, at + (c * TPR + t) * 8, cols - (c * TPR + t) * 8, v[c]);
+  }
+}
+
+// ---------------------------------------------------------------- sums and maxima over lanes, in every lane
+template <int N>
+__device__ __forceinline__ float rotated16(float v) {  // lane i of 16 sees lane (i - N) % 16
+  return __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(v), 0x120 + N, 0xf, 0xf, false));
+}
+__device__ __forceinline__ float sum16(float v) {
+  v += rotated16<8>(v);
+  v += rotated16<4>(v);
+  v += rotated16<2>(v);
+  return v + rotated16<1>(v);
+}
+__device__ __forceinline__ float max16(float v) {
+  v = fmaxf(v, rotated16<8>(v));
+  v = fmaxf(v, rotated16<4>(v));
+  v = fmaxf(v, rotated16<2>(v));
+  return fmaxf(v, rotated16<1>(v));
+}
+__device__ __forceinline__ float sum64(float v) {
+  v = sum16(v);
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return xhalf_sum(__uint_as_float(r[0]) + __uint_as_float(r[1]));
+}
+
+// ---------------------------------------------------------------- 8-bit blocks
+// A block's scale is 2^e with the smallest e that brings its largest finite magnitude within the type's range (448 =
+// 1.75 2^8, 57344 = 1.75 2^15), kept as the byte e + 127; an all-zero block has e = 0.  e stays at or above -127.
+__device__ __forceinline__ float finite_abs(float v) {
+  const float a = fabsf(v);
+  return a < __builtin_inff() ? a : 0.0f;
+}
+__device__ __forceinline__ int block_exponent(float amax, int fp8) {
+  const uint32_t u = __float_as_uint(amax);
+  const int e = (int)(u >> 23) - 127 - (fp8 == kFp8E4m3 ? 8 : 15) + ((u & 0x7fffffu) > 0x600000u ? 1 : 0);
+  return u == 0 ? 0 : max(e, -127);
+}
+__device__ __forceinline__ float power2(int e) {  // -127 <= e <= 127
+  return __uint_as_float(e > -127 ? (uint32_t)(e + 127) << 23 : 0x00400000u);
+}
+// Four values times 2^-e in 8 bits, to nearest even.  Non-finite values become NaN (e5m2 keeps infinities).
+__device__ __forceinline__ uint32_t cvt_fp8x4(float a, float b, float c, float d, int fp8) {
+  int w = 0;
+  if (fp8 == kFp8E4m3) {
+    w = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, w, false);
+    w = __builtin_amdgcn_cvt_pk_fp8_f32(c, d, w, true);
+  } else {
+    w = __builtin_amdgcn_cvt_pk_bf8_f32(a, b, w, false);
+    w = __builtin_amdgcn_cvt_pk_bf8_f32(c, d, w, true);
+  }
+  return (uint32_t)w;
+}
+__device__ __forceinline__ uint2 quantize8(const float (&f)[8], int e, int fp8) {
+  const float s = power2(-e);
+  return make_uint2(cvt_fp8x4(f[0] * s, f[1] * s, f[2] * s, f[3] * s, fp8),
+                    cvt_fp8x4(f[4] * s, f[5] * s, f[6] * s, f[7] * s, fp8));
+}
+
+}  // namespace svoo

@@ -1,0 +1,285 @@
+"""8-bit matrices with a power-of-two scale per block of 128, their product, and a linear layer on them with gradients.
+
+A block's scale is ``2^e`` with the smallest e that brings its largest magnitude within the type's range (448 for e4m3,
+57344 for e5m2), kept as an e8m0 byte (``torch.float8_e8m0fnu``).  Such a scale is exact to multiply by, and gfx950's
+matrix instructions apply it on the fly, so a product accumulates in fp32 inside the matrix unit over the whole
+contracted dimension.  A floating-point format loses no precision to it, only up to one binade of its range.
+
+Values of a matrix ``[.., K]`` are stored as ``[.., 128 ceil(K / 128)]`` (zeros past K) with scales ``[.., ceil(K / 128)]``:
+
+* :func:`fp8_quantize_rows`    a scale per 128 columns of each row (activations, gradients)
+* :func:`fp8_quantize_blocks`  a scale per 128 x 128 block (weights), also of the transpose
+* :func:`fp8_quantize_both`    rows, and the transposed matrix's rows: what a training step contracts both ways
+* :func:`fp8_dequantize`       the values back
+* :func:`fp8_matmul`           ``a b^T + bias``, with the tanh GELU if asked for
+* :func:`fp8_linear`           ``x W^T + b`` from 16 or 32-bit tensors, differentiable
+* :class:`Fp8Linear`           a ``torch.nn.Linear``'s stand-in for inference, its weight laid out once
+
+NaN stays NaN and infinities become NaN in e4m3 (e5m2 keeps them); they do not count towards a block's scale.
+"""
+
+from __future__ import annotations
+
+from typing import Optional, Tuple
+
+import torch
+
+from . import _lib
+
+FP8_TYPES = {torch.float8_e4m3fn: 0, torch.float8_e5m2: 1}
+SCALE_DTYPE = torch.float8_e8m0fnu
+BLOCK = 128
+_ACTS = {"none": 0, "gelu_tanh": 1}
+
+
+def _blocks(n: int) -> int:
+    return -(-n // BLOCK)
+
+
+def empty_fp8(lead, cols: int, dtype, device) -> torch.Tensor:
+    """Storage for the 8-bit values of ``[*lead, cols]``."""
+    return torch.empty(*lead, _blocks(cols) * BLOCK, dtype=dtype, device=device)
+
+
+def empty_scales(lead, cols: int, device) -> torch.Tensor:
+    return torch.empty(*lead, _blocks(cols), dtype=SCALE_DTYPE, device=device)
+
+
+def _fp8_type(dtype, name: str) -> int:
+    if dtype not in FP8_TYPES:
+        raise TypeError(f"{name}: float8_e4m3fn or float8_e5m2, got {dtype}")
+    return FP8_TYPES[dtype]
+
+
+def _matrix(x, name: str):
+    """``x [.., K]`` as ``(rows [M, K] with contiguous columns, its type)``, in place where the strides allow."""
+    kind = _lib.elem_type(x, name)
+    if x.dim() == 0 or x.shape[-1] == 0:
+        raise ValueError(f"{name}: shape {tuple(x.shape)}")
+    rows = x.reshape(x.numel() // x.shape[-1], x.shape[-1])
+    return (rows if rows.stride(1) == 1 else rows.contiguous()), kind
+
+
+def fp8_quantize_rows(x: torch.Tensor, dtype=torch.float8_e4m3fn) -> Tuple[torch.Tensor, torch.Tensor]:
+    """``x [.., K]`` to ``(q [.., Kp], s [.., Kb])``: a scale per 128 columns of each row.  No backward pass."""
+    _lib.refuse_grad("fp8_quantize_rows", x)
+    fp8 = _fp8_type(dtype, "fp8_quantize_rows")
+    rows, kind = _matrix(x, "x")
+    m, k = rows.shape
+    q, s = empty_fp8(x.shape[:-1], k, dtype, x.device), empty_scales(x.shape[:-1], k, x.device)
+    _lib.launch(x.device, "svoo_fp8_quantize_rows", rows.data_ptr(), kind, rows.stride(0), m, k, fp8, q.data_ptr(),
+                s.data_ptr())
+    return q, s
+
+
+def _tiles(rows, kind, dtype, square, plain, turned, sums=None):
+    """``svoo_fp8_quantize_tiles`` of ``rows [M, K]``: ``(q, s)`` if ``plain``, ``(qt, st)`` if ``turned``, column sums
+    into ``sums``."""
+    m, k = rows.shape
+    dev = rows.device
+    q = s = qt = st = ws = None
+    if plain:
+        q = empty_fp8((m,), k, dtype, dev)
+        s = empty_scales((_blocks(m) if square else m,), k, dev)
+    if turned:
+        qt = empty_fp8((k,), m, dtype, dev)
+        st = empty_scales((_blocks(k) if square else k,), m, dev)
+    if sums is not None:
+        ws = _lib.workspace(_lib.lib().svoo_fp8_quantize_tiles_workspace_size(m, k), dev)
+    _lib.launch(dev, "svoo_fp8_quantize_tiles", rows.data_ptr(), kind, rows.stride(0), m, k, FP8_TYPES[dtype],
+                int(square), _lib.ptr(q), _lib.ptr(s), _lib.ptr(qt), _lib.ptr(st), _lib.ptr(sums),
+                2 if sums is None else _lib.elem_type(sums, "sums"), _lib.ptr(ws), ws.numel() if ws is not None else 0)
+    return q, s, qt, st
+
+
+def fp8_quantize_blocks(w: torch.Tensor, dtype=torch.float8_e4m3fn, *, transposed: bool = False):
+    """``w [N, K]`` to ``(q [N, Kp], s [Nb, Kb])``: a scale per 128 x 128 block; with ``transposed`` also
+    ``(qt [K, Np], st [Kb, Nb])``, the same values and scales of the transpose.  No backward pass."""
+    _lib.refuse_grad("fp8_quantize_blocks", w)
+    _fp8_type(dtype, "fp8_quantize_blocks")
+    if w.dim() != 2:
+        raise ValueError(f"fp8_quantize_blocks: a matrix, got shape {tuple(w.shape)}")
+    rows, kind = _matrix(w, "w")
+    out = _tiles(rows, kind, dtype, True, True, transposed)
+    return out if transposed else out[:2]
+
+
+def fp8_quantize_both(x: torch.Tensor, dtype=torch.float8_e4m3fn):
+    """``x [M, K]`` to ``(q [M, Kp], s [M, Kb], qt [K, Mp], st [K, Mb])``: its rows and its transpose's rows, each with
+    a scale per 128 of its own columns, from one read.  No backward pass."""
+    _lib.refuse_grad("fp8_quantize_both", x)
+    _fp8_type(dtype, "fp8_quantize_both")
+    if x.dim() != 2:
+        raise ValueError(f"fp8_quantize_both: a matrix, got shape {tuple(x.shape)}")
+    rows, kind = _matrix(x, "x")
+    return _tiles(rows, kind, dtype, False, True, True)
+
+
+class _Operand:
+    """Checked 8-bit values and scales: ``rows [R, Kp]``, ``scales``, and the rows one scale covers."""
+
+    def __init__(self, q, s, name: str, dtypes, square: bool):
+        for t, n in ((q, name), (s, f"{name}'s scales")):
+            if not isinstance(t, torch.Tensor):
+                raise TypeError(f"{n}: a tensor, got {type(t).__name__}")
+        if q.dtype not in dtypes:
+            raise TypeError(f"{name}: {' or '.join(str(d)[6:] for d in dtypes)}, got {q.dtype}")
+        if s.dtype != SCALE_DTYPE:
+            raise TypeError(f"{name}'s scales: float8_e8m0fnu, got {s.dtype}")
+        _lib.require_gpu_tensor(q, name)
+        if s.device != q.device:
+            raise ValueError(f"{name}'s scales: on {s.device}, values on {q.device}")
+        if q.dim() < 1 or q.shape[-1] == 0 or q.shape[-1] % BLOCK:
+            raise ValueError(f"{name}: shape {tuple(q.shape)}; columns in whole blocks of {BLOCK} expected")
+        kb = q.shape[-1] // BLOCK
+        if tuple(s.shape) == (*q.shape[:-1], kb):
+            self.tall = 1
+        elif square and q.dim() == 2 and tuple(s.shape) == (_blocks(q.shape[0]), kb):
+            self.tall = BLOCK
+        else:
+            raise ValueError(f"{name}'s scales: shape {tuple(s.shape)} for values {tuple(q.shape)}")
+        self.lead, self.kp = q.shape[:-1], q.shape[-1]
+        n = q.numel() // self.kp
+        self.fp8 = FP8_TYPES[q.dtype]
+        q = q.view(torch.uint8).reshape(n, self.kp)
+        if q.stride(1) != 1 or q.stride(0) % 16 or q.data_ptr() % 16:
+            q = q.clone(memory_format=torch.contiguous_format)
+        s = s.view(torch.uint8).reshape(-1, kb)
+        self.q, self.s = q, s if s.stride(1) == 1 else s.contiguous()
+
+    def args(self):
+        return self.q.data_ptr(), self.q.stride(0), self.s.data_ptr(), self.s.stride(0)
+
+
+def fp8_dequantize(q: torch.Tensor, s: torch.Tensor, cols: Optional[int] = None, out_dtype=torch.bfloat16) -> torch.Tensor:
+    """The values ``[.., cols]`` (all stored columns by default) that 8-bit values and their scales stand for, rounded to
+    ``out_dtype``.  ``s`` has a row for each row of q, or for each 128 of a matrix's rows."""
+    o = _Operand(q, s, "q", tuple(FP8_TYPES), True)
+    cols = o.kp if cols is None else int(cols)
+    if not o.kp - BLOCK < cols <= o.kp:
+        raise ValueError(f"fp8_dequantize: cols={cols} of {o.kp} stored")
+    y = torch.empty(*o.lead, cols, dtype=out_dtype, device=q.device)
+    kind = _lib.elem_type(y, "out_dtype")
+    _lib.launch(q.device, "svoo_fp8_dequantize", *o.args(), o.tall, o.q.shape[0], cols, o.fp8, y.data_ptr(), kind)
+    return y
+
+
+def fp8_matmul(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: torch.Tensor,
+               bias: Optional[torch.Tensor] = None, activation: str = "none", out_dtype=torch.bfloat16) -> torch.Tensor:
+    """``act(a b^T + bias)`` of ``a [.., Kp]`` (e4m3 or e5m2, a scale per row and block) and ``b [N, Kp]`` (e4m3, a scale
+    per row or per 128 rows and block), accumulated in fp32 and rounded once to ``out_dtype``: ``[.., N]``.
+
+    ``activation``: ``"none"`` or ``"gelu_tanh"``.  The same call gives the same bits.  No backward pass."""
+    _lib.refuse_grad("fp8_matmul", bias)
+    if activation not in _ACTS:
+        raise ValueError(f"fp8_matmul: activation {activation!r} ({', '.join(_ACTS)})")
+    oa = _Operand(a, a_scale, "a", tuple(FP8_TYPES), False)
+    ob = _Operand(b, b_scale, "b", (torch.float8_e4m3fn,), True)
+    if b.dim() != 2 or oa.kp != ob.kp or b.device != a.device:
+        raise ValueError(f"fp8_matmul: a {tuple(a.shape)} on {a.device}, b {tuple(b.shape)} on {b.device}")
+    m, n = oa.q.shape[0], ob.q.shape[0]
+    bias_type = 2
+    if bias is not None:
+        bias_type = _lib.elem_type(bias, "bias")
+        if tuple(bias.shape) != (n,) or bias.device != a.device:
+            raise ValueError(f"bias: shape {tuple(bias.shape)} on {bias.device}; [{n}] on {a.device} expected")
+        bias = bias.contiguous()
+    c = torch.empty(*oa.lead, n, dtype=out_dtype, device=a.device)
+    kind = _lib.elem_type(c, "out_dtype")
+    need = _lib.lib().svoo_fp8_matmul_workspace_size(m, n, oa.kp)
+    ws = _lib.workspace(need, a.device) if need else None
+    _lib.launch(a.device, "svoo_fp8_matmul", *oa.args(), oa.fp8, *ob.args(), ob.tall, _lib.ptr(bias), bias_type,
+                _ACTS[activation], m, n, oa.kp, c.data_ptr(), kind, _lib.ptr(ws), need)
+    return c
+
+
+class _Linear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, grad_dtype):
+        rows, kind = _matrix(x, "x")
+        w, w_kind = _matrix(weight, "weight")
+        need_x, need_w = ctx.needs_input_grad[:2]
+        wq, ws, wqt, wst = _tiles(w, w_kind, torch.float8_e4m3fn, True, True, need_x)
+        if need_w:
+            q, s, qt, st = _tiles(rows, kind, torch.float8_e4m3fn, False, True, True)
+        else:
+            (q, s), qt, st = fp8_quantize_rows(rows), None, None
+        y = fp8_matmul(q, s, wq, ws, bias, out_dtype=x.dtype)
+        ctx.save_for_backward(wqt, wst, qt, st)
+        ctx.meta = x.shape, x.dtype, weight.shape, weight.dtype, None if bias is None else bias.dtype, grad_dtype
+        return y.view(*x.shape[:-1], w.shape[0])
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x_shape, x_dtype, w_shape, w_dtype, b_dtype, grad_dtype = ctx.meta
+        wqt, wst, qt, st = ctx.saved_tensors
+        need_x, need_w, need_b = ctx.needs_input_grad[:3]
+        need_b = need_b and b_dtype is not None
+        rows, kind = _matrix(dy, "dy")
+        dx = dw = db = None
+        if rows.shape[0] == 0:
+            dx = torch.empty(x_shape, dtype=x_dtype, device=dy.device) if need_x else None
+            dw = torch.zeros(w_shape, dtype=w_dtype, device=dy.device) if need_w else None
+            db = torch.zeros(w_shape[0], dtype=b_dtype, device=dy.device) if need_b else None
+            return dx, dw, db, None
+        if need_b:
+            db = torch.empty(w_shape[0], dtype=b_dtype, device=dy.device)
+        q, s, gt, gs = _tiles(rows, kind, grad_dtype, False, need_x, need_w, db)
+        if need_x:
+            dx = fp8_matmul(q, s, wqt, wst, out_dtype=x_dtype).view(x_shape)
+        if need_w:
+            dw = fp8_matmul(gt, gs, qt, st, out_dtype=w_dtype)
+        return dx, dw, db, None
+
+
+def fp8_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None,
+               grad_dtype=torch.float8_e4m3fn) -> torch.Tensor:
+    """``x [.., K] @ weight [N, K]^T + bias`` with 8-bit operands: x in rows of 128, the weight in 128 x 128 blocks, both
+    e4m3.  Differentiable, once: ``dx`` from the incoming gradient's rows (``grad_dtype``: e4m3, or e5m2 for gradients
+    of a wide range) and the weight, ``dweight`` from the gradient's and x's columns in blocks of 128 rows, ``dbias`` in
+    fp32 sums of the unquantised gradient.  Results have the type of x, of weight and of bias.
+
+    Kept for the backward pass: 8-bit copies of x and of the weight."""
+    _fp8_type(grad_dtype, "fp8_linear")
+    _lib.elem_type(weight, "weight")
+    if weight.dim() != 2 or 0 in weight.shape or x.dim() == 0 or x.shape[-1] != weight.shape[1] or \
+            weight.device != x.device:
+        raise ValueError(f"fp8_linear: x {tuple(x.shape)} on {x.device}, weight {tuple(weight.shape)} on {weight.device}")
+    return _Linear.apply(x, weight, bias, grad_dtype)
+
+
+class Fp8Linear(torch.nn.Module):
+    """A linear layer for inference on 8-bit operands: the weight laid out once, x quantised in rows at every call.
+
+    Buffers hold bytes, so ``module.to(dtype)`` leaves them alone (it changes the bias, in whatever of bf16, fp16 and
+    fp32).  The output has x's type."""
+
+    def __init__(self, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, activation: str = "none"):
+        super().__init__()
+        if activation not in _ACTS:
+            raise ValueError(f"Fp8Linear: activation {activation!r} ({', '.join(_ACTS)})")
+        q, s = fp8_quantize_blocks(weight.detach())
+        self.out_features, self.in_features = weight.shape
+        self.activation = activation
+        self.register_buffer("weight_q", q.view(torch.uint8))
+        self.register_buffer("weight_scale", s.view(torch.uint8))
+        self.register_buffer("bias", None if bias is None else bias.detach().clone())
+
+    @classmethod
+    def from_linear(cls, linear: torch.nn.Linear, activation: str = "none") -> "Fp8Linear":
+        return cls(linear.weight, linear.bias, activation)
+
+    def forward_quantized(self, q: torch.Tensor, s: torch.Tensor, out_dtype=torch.bfloat16) -> torch.Tensor:
+        """The layer on rows that are quantised already (:func:`svoo_amd.norm.layer_norm_fp8`)."""
+        return fp8_matmul(q, s, self.weight_q.view(torch.float8_e4m3fn), self.weight_scale.view(SCALE_DTYPE),
+                          bias=self.bias, activation=self.activation, out_dtype=out_dtype)
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        if x.dim() == 0 or x.shape[-1] != self.in_features:
+            raise ValueError(f"Fp8Linear: x {tuple(x.shape)} for {self.in_features} inputs")
+        return self.forward_quantized(*fp8_quantize_rows(x), out_dtype=x.dtype)
+
+    def extra_repr(self) -> str:
+        return f"in_features={self.in_features}, out_features={self.out_features}, bias={self.bias is not None}, " \
+               f"activation={self.activation}"
