@@ -66,10 +66,11 @@ _SIGS = {
     "svoo_fp8_quantize_tiles_workspace_size": (c_size_t, [c_longlong, c_longlong]),
     "svoo_fp8_quantize_tiles": (c_int, [P, c_int, c_longlong, c_longlong, c_longlong, c_int, c_int, P, P, P, P, P, c_int,
                                         P, c_size_t, P]),
-    "svoo_fp8_dequantize": (c_int, [P, c_longlong, P, c_longlong, c_int, c_longlong, c_longlong, c_int, P, c_int, P]),
-    "svoo_fp8_matmul_workspace_size": (c_size_t, [c_longlong, c_longlong, c_longlong]),
-    "svoo_fp8_matmul": (c_int, [P, c_longlong, P, c_longlong, c_int, P, c_longlong, P, c_longlong, c_int, P, c_int, c_int,
-                                c_longlong, c_longlong, c_longlong, P, c_int, P, c_size_t, P]),
+    "svoo_fp8_dequantize": (c_int, [P, c_longlong, P, c_longlong, c_longlong, c_int, c_longlong, c_longlong, c_int, P, c_int,
+                                    P]),
+    "svoo_fp8_matmul_workspace_size": (c_size_t, [c_longlong, c_longlong, c_longlong, c_int]),
+    "svoo_fp8_matmul": (c_int, [P, c_longlong, P, c_longlong, c_longlong, c_int, P, c_longlong, P, c_longlong, c_longlong,
+                                c_int, P, c_int, c_int, c_longlong, c_longlong, c_longlong, P, c_int, P, c_size_t, P]),
     "svoo_vbsa_ear_fwd": (c_int, [P, P, P, P, P, P, P, P, P, c_int, c_int, c_int, c_int, c_int, P, c_size_t, P, P]),
 }
 

@@ -20,9 +20,9 @@ struct QuantArgs {
   int rows, cols;
   int fp8;
   uint8_t* q;          // [rows][row_blocks * 128] or null
-  uint8_t* scale;      // [rows][row_blocks], or [col_blocks][row_blocks] for square blocks
+  uint8_t* scale;      // [row_blocks][rows], or [col_blocks][row_blocks] for square blocks
   uint8_t* qt;         // [cols][col_blocks * 128] or null
-  uint8_t* scale_t;    // [cols][col_blocks], or [row_blocks][col_blocks]
+  uint8_t* scale_t;    // [col_blocks][cols], or [row_blocks][col_blocks]
   float* col_sums;     // [col_blocks][cols] or null
   int row_blocks, col_blocks;  // blocks of 128 columns in a row, of 128 rows in a column
 };
@@ -49,7 +49,10 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(QuantArgs a) {
       const int e8 = block_exponent(max16(amax), a.fp8);
       if (u < units) {
         *(uint2*)(a.q + (size_t)u * 128 + t * 8) = quantize8(f[i], e8, a.fp8);
-        if (t == 0) a.scale[u] = (uint8_t)(e8 + 127);
+        if (t == 0) {
+          const unsigned row = u / a.row_blocks;
+          a.scale[(size_t)(u - row * a.row_blocks) * a.rows + row] = (uint8_t)(e8 + 127);
+        }
       }
     }
   }
@@ -99,7 +102,7 @@ __global__ void __launch_bounds__(256) quantize_tile_kernel(QuantArgs a) {
       }
       if (row0 + i < a.rows) {
         *(uint2*)(a.q + ((size_t)(row0 + i) * a.row_blocks + blockIdx.x) * 128 + t * 8) = quantize8(f[i], e8, a.fp8);
-        if (!kSquare && t == 0) a.scale[(size_t)(row0 + i) * a.row_blocks + blockIdx.x] = (uint8_t)(e8 + 127);
+        if (!kSquare && t == 0) a.scale[(size_t)blockIdx.x * a.rows + row0 + i] = (uint8_t)(e8 + 127);
       }
     }
   }
@@ -145,7 +148,7 @@ __global__ void __launch_bounds__(256) quantize_tile_kernel(QuantArgs a) {
       for (int k = 0; k < 16; ++k) v = fmaxf(v, ((const float*)col_part[k])[threadIdx.x]);
       const int e8 = block_exponent(v, a.fp8), col = blockIdx.x * 128 + threadIdx.x;
       col_exp[threadIdx.x] = e8;
-      if (col < a.cols) a.scale_t[(size_t)col * a.col_blocks + blockIdx.y] = (uint8_t)(e8 + 127);
+      if (col < a.cols) a.scale_t[(size_t)blockIdx.y * a.cols + col] = (uint8_t)(e8 + 127);
     }
     __syncthreads();
 #pragma unroll
@@ -192,7 +195,7 @@ struct DequantArgs {
   const uint8_t* q;
   long long q_row;
   const uint8_t* scale;
-  long long scale_row;
+  long long scale_row, scale_col;
   int tall;            // rows per scale
   int rows, cols, fp8;
   void* y;             // [rows][cols]
@@ -211,7 +214,7 @@ __global__ void __launch_bounds__(256) dequantize_kernel(DequantArgs a) {
       const unsigned v = min(v0 + i * step, total - 1), row = v / a.vecs;
       const int col = (v - row * a.vecs) * 8;
       w[i] = *(const uint2*)(a.q + row * a.q_row + col);
-      byte[i] = a.scale[(row / a.tall) * a.scale_row + col / 128];
+      byte[i] = a.scale[(row / a.tall) * a.scale_row + (col / 128) * a.scale_col];
     }
 #pragma unroll
     for (int i = 0; i < kUnroll; ++i) {
@@ -314,8 +317,8 @@ extern "C" int svoo_fp8_quantize_tiles(const void* x, int type, long long x_row_
 }
 
 extern "C" int svoo_fp8_dequantize(const uint8_t* q, long long q_row_stride, const uint8_t* scale,
-                                   long long scale_row_stride, int rows_per_scale, long long rows, long long cols,
-                                   int fp8_type, void* y, int type, void* stream) {
+                                   long long scale_row_stride, long long scale_col_stride, int rows_per_scale,
+                                   long long rows, long long cols, int fp8_type, void* y, int type, void* stream) {
   static const char* name = "svoo_fp8_dequantize";
   if (const int rc = check_matrix(name, type, fp8_type, rows, cols)) return rc;
   SVOO_REQUIRE(rows_per_scale == 1 || rows_per_scale == 128, SVOO_ERR_INVALID_ARG, "%s: %d rows a scale (1 or 128)", name,
@@ -326,7 +329,8 @@ extern "C" int svoo_fp8_dequantize(const uint8_t* q, long long q_row_stride, con
                "%s: rows of q must start at 8-byte addresses", name);
   const int vecs = (int)((cols + 7) / 8);
   SVOO_REQUIRE(rows * vecs < (1ll << 31), SVOO_ERR_UNSUPPORTED, "%s: %lld x %lld", name, rows, cols);
-  const DequantArgs a = {q, q_row_stride, scale, scale_row_stride, rows_per_scale, (int)rows, (int)cols, fp8_type, y, vecs};
+  const DequantArgs a = {q, q_row_stride, scale, scale_row_stride, scale_col_stride, rows_per_scale, (int)rows, (int)cols, fp8_type, y,
+                         vecs};
   const unsigned blocks = (unsigned)std::min((rows * vecs + 255) / 256, 4096ll);
   for_type(type, [&](auto t) {
     hipLaunchKernelGGL(dequantize_kernel<decltype(t)::value>, dim3(blocks), dim3(256), 0, (hipStream_t)stream, a);

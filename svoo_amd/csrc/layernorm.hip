@@ -137,7 +137,7 @@ __global__ void __launch_bounds__(TPR > 256 ? TPR : 256) norm_fwd_kernel(NormArg
         const int e8 = block_exponent(max16(amax), a.fp8);
         if (col < blocks * 128) {
           *(uint2*)(a.q + (size_t)row * blocks * 128 + col) = quantize8(x[c], e8, a.fp8);
-          if (t % 16 == 0) a.q_scale[(size_t)row * blocks + col / 128] = (uint8_t)(e8 + 127);
+          if (t % 16 == 0) a.q_scale[(size_t)(col / 128) * a.rows + row] = (uint8_t)(e8 + 127);
         }
       }
     }

@@ -12,6 +12,7 @@ enum Fp8Type { kFp8E4m3 = 0, kFp8E5m2 = 1 };
 // Four dwords at any byte address (gfx950's global loads and stores need no alignment).
 struct __attribute__((packed, aligned(1))) Dwords4 { u32x4_t v; };
 struct __attribute__((packed, aligned(1))) Dwords2 { uint32_t v[2]; };
+struct __attribute__((packed, aligned(1))) Dword { uint32_t v; };
 
 __device__ __forceinline__ float row_elem(const void* p, int type, long long i) {
   if (type == kRowBf16) return bf16_to_f32(((const uint16_t*)p)[i]);

@@ -20,6 +20,7 @@ NaN stays NaN and infinities become NaN in e4m3 (e5m2 keeps them); they do not c
 
 from __future__ import annotations
 
+import math
 from typing import Optional, Tuple
 
 import torch
@@ -42,7 +43,12 @@ def empty_fp8(lead, cols: int, dtype, device) -> torch.Tensor:
 
 
 def empty_scales(lead, cols: int, device) -> torch.Tensor:
-    return torch.empty(*lead, _blocks(cols), dtype=SCALE_DTYPE, device=device)
+    """Scales ``[*lead, ceil(cols / 128)]`` of rows, stored with neighbouring rows side by side."""
+    return torch.empty(_blocks(cols), math.prod(lead), dtype=SCALE_DTYPE, device=device).t().view(*lead, _blocks(cols))
+
+
+def _square_scales(rows: int, cols: int, device) -> torch.Tensor:
+    return torch.empty(_blocks(rows), _blocks(cols), dtype=SCALE_DTYPE, device=device)
 
 
 def _fp8_type(dtype, name: str) -> int:
@@ -80,10 +86,10 @@ def _tiles(rows, kind, dtype, square, plain, turned, sums=None):
     q = s = qt = st = ws = None
     if plain:
         q = empty_fp8((m,), k, dtype, dev)
-        s = empty_scales((_blocks(m) if square else m,), k, dev)
+        s = _square_scales(m, k, dev) if square else empty_scales((m,), k, dev)
     if turned:
         qt = empty_fp8((k,), m, dtype, dev)
-        st = empty_scales((_blocks(k) if square else k,), m, dev)
+        st = _square_scales(k, m, dev) if square else empty_scales((k,), m, dev)
     if sums is not None:
         ws = _lib.workspace(_lib.lib().svoo_fp8_quantize_tiles_workspace_size(m, k), dev)
     _lib.launch(dev, "svoo_fp8_quantize_tiles", rows.data_ptr(), kind, rows.stride(0), m, k, FP8_TYPES[dtype],
@@ -142,13 +148,19 @@ class _Operand:
         n = q.numel() // self.kp
         self.fp8 = FP8_TYPES[q.dtype]
         q = q.view(torch.uint8).reshape(n, self.kp)
-        if q.stride(1) != 1 or q.stride(0) % 16 or q.data_ptr() % 16:
+        if q.stride(1) != 1 or q.data_ptr() % 16 or (n > 1 and (q.stride(0) % 16 or q.stride(0) < self.kp)):
             q = q.clone(memory_format=torch.contiguous_format)
-        s = s.view(torch.uint8).reshape(-1, kb)
-        self.q, self.s = q, s if s.stride(1) == 1 else s.contiguous()
+        self.row = q.stride(0) if n > 1 else self.kp
+        self.q, self.s = q, s.view(torch.uint8).reshape(n if self.tall == 1 else -1, kb)
+
+    def rows_side_by_side(self):
+        """Row scales as a product reads them: those of neighbouring rows in neighbouring bytes."""
+        if self.tall == 1 and self.s.stride(0) != 1:
+            self.s = self.s.t().contiguous().t()
+        return self
 
     def args(self):
-        return self.q.data_ptr(), self.q.stride(0), self.s.data_ptr(), self.s.stride(0)
+        return self.q.data_ptr(), self.row, self.s.data_ptr(), self.s.stride(0), self.s.stride(1)
 
 
 def fp8_dequantize(q: torch.Tensor, s: torch.Tensor, cols: Optional[int] = None, out_dtype=torch.bfloat16) -> torch.Tensor:
@@ -173,8 +185,8 @@ def fp8_matmul(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale:
     _lib.refuse_grad("fp8_matmul", bias)
     if activation not in _ACTS:
         raise ValueError(f"fp8_matmul: activation {activation!r} ({', '.join(_ACTS)})")
-    oa = _Operand(a, a_scale, "a", tuple(FP8_TYPES), False)
-    ob = _Operand(b, b_scale, "b", (torch.float8_e4m3fn,), True)
+    oa = _Operand(a, a_scale, "a", tuple(FP8_TYPES), False).rows_side_by_side()
+    ob = _Operand(b, b_scale, "b", (torch.float8_e4m3fn,), True).rows_side_by_side()
     if b.dim() != 2 or oa.kp != ob.kp or b.device != a.device:
         raise ValueError(f"fp8_matmul: a {tuple(a.shape)} on {a.device}, b {tuple(b.shape)} on {b.device}")
     m, n = oa.q.shape[0], ob.q.shape[0]
@@ -186,7 +198,7 @@ def fp8_matmul(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale:
         bias = bias.contiguous()
     c = torch.empty(*oa.lead, n, dtype=out_dtype, device=a.device)
     kind = _lib.elem_type(c, "out_dtype")
-    need = _lib.lib().svoo_fp8_matmul_workspace_size(m, n, oa.kp)
+    need = _lib.lib().svoo_fp8_matmul_workspace_size(m, n, oa.kp, kind)
     ws = _lib.workspace(need, a.device) if need else None
     _lib.launch(a.device, "svoo_fp8_matmul", *oa.args(), oa.fp8, *ob.args(), ob.tall, _lib.ptr(bias), bias_type,
                 _ACTS[activation], m, n, oa.kp, c.data_ptr(), kind, _lib.ptr(ws), need)

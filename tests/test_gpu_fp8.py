@@ -124,7 +124,9 @@ SHAPES = [(1, 1, 128), (1, 9216, 1536), (1, 333, 200), (2, 130, 4096), (5, 64, 3
           (17, 96, 128), (31, 40, 2048), (33, 513, 896), (64, 64, 128), (65, 200, 300), (100, 1536, 512), (128, 128, 8960),
           (129, 129, 129), (200, 777, 256), (255, 300, 1000), (256, 256, 256), (257, 511, 384), (512, 1536, 1024),
           (513, 1025, 640), (1000, 1000, 1000), (1013, 333, 2000), (2048, 512, 128), (3000, 2000, 500), (4100, 1030, 300),
-          (8200, 264, 136), (333, 1000, 33000)]
+          (8200, 264, 136), (333, 1000, 33000),
+          # enough tiles for the 256 x 256 kernel: edges in both directions, odd columns, one to many stages and shares
+          (16300, 4224, 300), (9000, 9007, 128), (5120, 5000, 1100), (7777, 5121, 640), (1500, 1290, 20100)]
 
 
 @pytest.mark.parametrize("m,n,k", SHAPES)

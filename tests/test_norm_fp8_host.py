@@ -51,15 +51,15 @@ def test_entries_with_nothing_to_do_launch_nothing():
     assert _call("svoo_layer_norm_bwd", BWD, dict(rows=0, dw=None, db=None), list(BWD))[0] == 0
     assert _call("svoo_layer_norm_bwd", BWD, dict(dx=None, dw=None, db=None), list(BWD))[0] == 0
     assert lib.svoo_fp8_quantize_rows(None, 0, 64, 0, 64, 0, None, None, None) == 0
-    assert lib.svoo_fp8_dequantize(None, 128, None, 1, 1, 0, 64, 0, None, 0, None) == 0
-    assert lib.svoo_fp8_matmul(None, 128, None, 1, 0, None, 128, None, 1, 1, None, 0, 0, 0, 5, 128, None, 0, None, 0, None) == 0
+    assert lib.svoo_fp8_dequantize(None, 128, None, 1, 1, 1, 0, 64, 0, None, 0, None) == 0
+    assert lib.svoo_fp8_matmul(None, 128, None, 1, 1, 0, None, 128, None, 1, 1, 1, None, 0, 0, 0, 5, 128, None, 0, None, 0, None) == 0
     assert lib.svoo_layer_norm_bwd_workspace_size(0, 5, 5) == 0
     assert lib.svoo_layer_norm_bwd_workspace_size(1, 1, 64) == 0  # one part writes its gradients itself
     assert lib.svoo_layer_norm_bwd_workspace_size(1, 32760, 1536) <= 1 << 24
     assert lib.svoo_fp8_quantize_tiles_workspace_size(129, 100) == 800
 
 
-MM = dict(a=16, ar=128, sa=16, sar=1, a_type=0, b=16, br=128, sb=16, sbr=1, tall=128, bias=None, bias_type=0, act=0, m=4, n=4,
+MM = dict(a=16, ar=128, sa=16, sar=1, sac=4, a_type=0, b=16, br=128, sb=16, sbr=1, sbc=1, tall=128, bias=None, bias_type=0, act=0, m=4, n=4,
           k=128, c=16, c_type=0, ws=None, ws_bytes=0)
 
 
@@ -97,8 +97,8 @@ def test_row_quantiser_and_dequantiser_entry_refusals():
     for args, message in (((16, 7, 64, 4, 64, 0, 16, 16, None), "element type 7"), ((16, 0, 64, 4, 64, 0, 4, 16, None), "8-byte"),
                           ((16, 0, 64, 4, 64, 0, None, 16, None), "null"), ((16, 0, 64, -4, 64, 0, 16, 16, None), "-4 x 64")):
         assert lib.svoo_fp8_quantize_rows(*args) == -1 and message in _lib.last_error()
-    for args, message in (((16, 128, 16, 1, 7, 4, 64, 0, 16, 0, None), "7 rows a scale"),
-                          ((16, 12, 16, 1, 1, 4, 64, 0, 16, 0, None), "8-byte"), ((16, 128, None, 1, 1, 4, 64, 0, 16, 0, None), "null")):
+    for args, message in (((16, 128, 16, 1, 1, 7, 4, 64, 0, 16, 0, None), "7 rows a scale"),
+                          ((16, 12, 16, 1, 1, 1, 4, 64, 0, 16, 0, None), "8-byte"), ((16, 128, None, 1, 1, 1, 4, 64, 0, 16, 0, None), "null")):
         assert lib.svoo_fp8_dequantize(*args) == -1 and message in _lib.last_error()
 
 
