@@ -109,14 +109,25 @@ def call(name: str, *args) -> None:
         raise RuntimeError(f"{name} failed ({rc}): {last_error()}")
 
 
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
+def raw_stream(index: int) -> int:
+    """The current HIP stream of device ``index`` as an integer handle, without making a stream object of it."""
+    return _raw_stream(index) if _raw_stream is not None else torch.cuda.current_stream(index).cuda_stream
+
+
 def launch(device: torch.device, name: str, *args) -> None:
     """:func:`call` with the current stream of ``device`` as the last argument, on that device (a launch goes to the
     current one)."""
-    if device.index == torch.cuda.current_device():
-        call(name, *args, stream_of(device))
+    index = device.index
+    if index == torch.cuda.current_device():
+        rc = getattr(_lib or lib(), name)(*args, raw_stream(index))
     else:
         with torch.cuda.device(device):
-            call(name, *args, stream_of(device))
+            rc = getattr(lib(), name)(*args, raw_stream(index))
+    if rc != 0:
+        raise RuntimeError(f"{name} failed ({rc}): {last_error()}")
 
 
 def ptr(t: Optional[torch.Tensor]) -> Optional[int]:
@@ -164,7 +175,9 @@ def elem_type(t: torch.Tensor, name: str) -> int:
 
 def refuse_grad(name: str, *tensors) -> None:
     """An operator without a backward pass takes no tensor that waits for a gradient: its result would end the graph."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+    if not torch.is_grad_enabled():
+        return
+    if any(t is not None and t.requires_grad for t in tensors):
         raise RuntimeError(f"{name} has no backward pass: call it under torch.no_grad() or on detached tensors")
 
 

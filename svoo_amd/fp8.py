@@ -30,6 +30,7 @@ from . import _lib
 FP8_TYPES = {torch.float8_e4m3fn: 0, torch.float8_e5m2: 1}
 SCALE_DTYPE = torch.float8_e8m0fnu
 BLOCK = 128
+_BOTH, _E4M3 = tuple(FP8_TYPES), (torch.float8_e4m3fn,)
 _ACTS = {"none": 0, "gelu_tanh": 1}
 
 
@@ -39,12 +40,15 @@ def _blocks(n: int) -> int:
 
 def empty_fp8(lead, cols: int, dtype, device) -> torch.Tensor:
     """Storage for the 8-bit values of ``[*lead, cols]``."""
-    return torch.empty(*lead, _blocks(cols) * BLOCK, dtype=dtype, device=device)
+    return torch.empty((*lead, _blocks(cols) * BLOCK), dtype=dtype, device=device)
 
 
 def empty_scales(lead, cols: int, device) -> torch.Tensor:
     """Scales ``[*lead, ceil(cols / 128)]`` of rows, stored with neighbouring rows side by side."""
-    return torch.empty(_blocks(cols), math.prod(lead), dtype=SCALE_DTYPE, device=device).t().view(*lead, _blocks(cols))
+    kb = _blocks(cols)
+    if len(lead) == 1:
+        return torch.empty_strided((lead[0], kb), (1, max(lead[0], 1)), dtype=SCALE_DTYPE, device=device)
+    return torch.empty(kb, math.prod(lead), dtype=SCALE_DTYPE, device=device).t().view(*lead, kb)
 
 
 def _square_scales(rows: int, cols: int, device) -> torch.Tensor:
@@ -60,10 +64,12 @@ def _fp8_type(dtype, name: str) -> int:
 def _matrix(x, name: str):
     """``x [.., K]`` as ``(rows [M, K] with contiguous columns, its type)``, in place where the strides allow."""
     kind = _lib.elem_type(x, name)
-    if x.dim() == 0 or x.shape[-1] == 0:
+    dims = x.dim()
+    if dims == 0 or x.shape[-1] == 0:
         raise ValueError(f"{name}: shape {tuple(x.shape)}")
-    rows = x.reshape(x.numel() // x.shape[-1], x.shape[-1])
-    return (rows if rows.stride(1) == 1 else rows.contiguous()), kind
+    if dims != 2:
+        x = x.reshape(x.numel() // x.shape[-1], x.shape[-1])
+    return (x if x.stride(1) == 1 or x.shape[1] == 1 else x.contiguous()), kind
 
 
 def fp8_quantize_rows(x: torch.Tensor, dtype=torch.float8_e4m3fn) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -122,57 +128,59 @@ def fp8_quantize_both(x: torch.Tensor, dtype=torch.float8_e4m3fn):
 
 
 class _Operand:
-    """Checked 8-bit values and scales: ``rows [R, Kp]``, ``scales``, and the rows one scale covers."""
+    """Checked 8-bit values and scales, as the C entries take them."""
 
-    def __init__(self, q, s, name: str, dtypes, square: bool):
-        for t, n in ((q, name), (s, f"{name}'s scales")):
-            if not isinstance(t, torch.Tensor):
-                raise TypeError(f"{n}: a tensor, got {type(t).__name__}")
+    __slots__ = ("lead", "kp", "rows", "fp8", "tall", "args", "keep")
+
+    def __init__(self, q, s, name: str, dtypes, square: bool, side_by_side: bool = False):
+        """``square``: one scale may cover 128 rows.  ``side_by_side``: row scales are wanted with neighbouring rows in
+        neighbouring bytes, and laid out so if they are not."""
+        if not isinstance(q, torch.Tensor) or not isinstance(s, torch.Tensor):
+            raise TypeError(f"{name}: tensors of values and scales, got {type(q).__name__}, {type(s).__name__}")
         if q.dtype not in dtypes:
             raise TypeError(f"{name}: {' or '.join(str(d)[6:] for d in dtypes)}, got {q.dtype}")
         if s.dtype != SCALE_DTYPE:
             raise TypeError(f"{name}'s scales: float8_e8m0fnu, got {s.dtype}")
-        _lib.require_gpu_tensor(q, name)
+        if not q.is_cuda:
+            _lib.require_gpu_tensor(q, name)
         if s.device != q.device:
             raise ValueError(f"{name}'s scales: on {s.device}, values on {q.device}")
-        if q.dim() < 1 or q.shape[-1] == 0 or q.shape[-1] % BLOCK:
-            raise ValueError(f"{name}: shape {tuple(q.shape)}; columns in whole blocks of {BLOCK} expected")
-        kb = q.shape[-1] // BLOCK
-        if tuple(s.shape) == (*q.shape[:-1], kb):
+        shape, s_shape = q.shape, s.shape
+        dims = len(shape)
+        self.lead, kp = shape[:-1], shape[-1] if dims else 0
+        if kp == 0 or kp % BLOCK:
+            raise ValueError(f"{name}: shape {tuple(shape)}; columns in whole blocks of {BLOCK} expected")
+        kb = kp // BLOCK
+        if s_shape == (*self.lead, kb):
             self.tall = 1
-        elif square and q.dim() == 2 and tuple(s.shape) == (_blocks(q.shape[0]), kb):
+        elif square and dims == 2 and s_shape == (_blocks(shape[0]), kb):
             self.tall = BLOCK
         else:
-            raise ValueError(f"{name}'s scales: shape {tuple(s.shape)} for values {tuple(q.shape)}")
-        self.lead, self.kp = q.shape[:-1], q.shape[-1]
-        n = q.numel() // self.kp
-        self.fp8 = FP8_TYPES[q.dtype]
-        q = q.view(torch.uint8).reshape(n, self.kp)
-        if q.stride(1) != 1 or q.data_ptr() % 16 or (n > 1 and (q.stride(0) % 16 or q.stride(0) < self.kp)):
-            q = q.clone(memory_format=torch.contiguous_format)
-        self.row = q.stride(0) if n > 1 else self.kp
-        self.q, self.s = q, s.view(torch.uint8).reshape(n if self.tall == 1 else -1, kb)
-
-    def rows_side_by_side(self):
-        """Row scales as a product reads them: those of neighbouring rows in neighbouring bytes."""
-        if self.tall == 1 and self.s.stride(0) != 1:
-            self.s = self.s.t().contiguous().t()
-        return self
-
-    def args(self):
-        return self.q.data_ptr(), self.row, self.s.data_ptr(), self.s.stride(0), self.s.stride(1)
+            raise ValueError(f"{name}'s scales: shape {tuple(s_shape)} for values {tuple(shape)}")
+        if dims != 2:
+            n = math.prod(self.lead)
+            q, s = q.reshape(n, kp), s.view(torch.uint8).reshape(n, kb)
+        self.kp, self.rows, self.fp8 = kp, q.shape[0], FP8_TYPES[q.dtype]
+        row, at = q.stride(0) if self.rows > 1 else kp, q.data_ptr()
+        if q.stride(1) != 1 or at % 16 or row % 16 or row < kp:
+            q = q.view(torch.uint8).clone(memory_format=torch.contiguous_format)
+            row, at = kp, q.data_ptr()
+        if side_by_side and self.tall == 1 and self.rows > 1 and s.stride(0) != 1:
+            s = s.view(torch.uint8).t().contiguous().t()
+        self.keep = q, s
+        self.args = at, row, s.data_ptr(), s.stride(0) if s.shape[0] > 1 else 1, s.stride(1) if kb > 1 else s.shape[0]
 
 
 def fp8_dequantize(q: torch.Tensor, s: torch.Tensor, cols: Optional[int] = None, out_dtype=torch.bfloat16) -> torch.Tensor:
     """The values ``[.., cols]`` (all stored columns by default) that 8-bit values and their scales stand for, rounded to
     ``out_dtype``.  ``s`` has a row for each row of q, or for each 128 of a matrix's rows."""
-    o = _Operand(q, s, "q", tuple(FP8_TYPES), True)
+    o = _Operand(q, s, "q", _BOTH, True)
     cols = o.kp if cols is None else int(cols)
     if not o.kp - BLOCK < cols <= o.kp:
         raise ValueError(f"fp8_dequantize: cols={cols} of {o.kp} stored")
     y = torch.empty(*o.lead, cols, dtype=out_dtype, device=q.device)
     kind = _lib.elem_type(y, "out_dtype")
-    _lib.launch(q.device, "svoo_fp8_dequantize", *o.args(), o.tall, o.q.shape[0], cols, o.fp8, y.data_ptr(), kind)
+    _lib.launch(q.device, "svoo_fp8_dequantize", *o.args, o.tall, o.rows, cols, o.fp8, y.data_ptr(), kind)
     return y
 
 
@@ -185,22 +193,22 @@ def fp8_matmul(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale:
     _lib.refuse_grad("fp8_matmul", bias)
     if activation not in _ACTS:
         raise ValueError(f"fp8_matmul: activation {activation!r} ({', '.join(_ACTS)})")
-    oa = _Operand(a, a_scale, "a", tuple(FP8_TYPES), False).rows_side_by_side()
-    ob = _Operand(b, b_scale, "b", (torch.float8_e4m3fn,), True).rows_side_by_side()
+    oa = _Operand(a, a_scale, "a", _BOTH, False, True)
+    ob = _Operand(b, b_scale, "b", _E4M3, True, True)
     if b.dim() != 2 or oa.kp != ob.kp or b.device != a.device:
         raise ValueError(f"fp8_matmul: a {tuple(a.shape)} on {a.device}, b {tuple(b.shape)} on {b.device}")
-    m, n = oa.q.shape[0], ob.q.shape[0]
+    m, n = oa.rows, ob.rows
     bias_type = 2
     if bias is not None:
         bias_type = _lib.elem_type(bias, "bias")
         if tuple(bias.shape) != (n,) or bias.device != a.device:
             raise ValueError(f"bias: shape {tuple(bias.shape)} on {bias.device}; [{n}] on {a.device} expected")
         bias = bias.contiguous()
-    c = torch.empty(*oa.lead, n, dtype=out_dtype, device=a.device)
+    c = torch.empty((*oa.lead, n), dtype=out_dtype, device=a.device)
     kind = _lib.elem_type(c, "out_dtype")
     need = _lib.lib().svoo_fp8_matmul_workspace_size(m, n, oa.kp, kind)
     ws = _lib.workspace(need, a.device) if need else None
-    _lib.launch(a.device, "svoo_fp8_matmul", *oa.args(), oa.fp8, *ob.args(), ob.tall, _lib.ptr(bias), bias_type,
+    _lib.launch(a.device, "svoo_fp8_matmul", *oa.args, oa.fp8, *ob.args, ob.tall, _lib.ptr(bias), bias_type,
                 _ACTS[activation], m, n, oa.kp, c.data_ptr(), kind, _lib.ptr(ws), need)
     return c
 

@@ -13,7 +13,7 @@ as 8-bit rows for :func:`svoo_amd.fp8.fp8_matmul` instead.
 
 from __future__ import annotations
 
-from typing import Optional, Tuple
+from typing import Optional, Sequence
 
 import torch
 
@@ -22,129 +22,158 @@ from .fp8 import FP8_TYPES, empty_fp8, empty_scales
 
 
 def _param(p, cols: int, batch: int, device, name: str):
-    """``p`` as ``(rows [1 or batch, cols], one row per batch entry?)``."""
-    if p is None:
-        return None, False
-    _lib.elem_type(p, name)
+    """``p`` as what the C entry takes: ``(pointer, type, elements between batch entries)``, with the tensor read (kept
+    alive by the caller)."""
+    kind = _lib.elem_type(p, name)
+    shape = p.shape
     if p.device != device:
         raise ValueError(f"{name}: on {p.device}, x on {device}")
-    if p.dim() == 0 or p.shape[-1] != cols or any(n != 1 for n in p.shape[1:-1]) or \
-            (p.dim() > 1 and p.shape[0] not in (1, batch)):
-        raise ValueError(f"{name}: shape {tuple(p.shape)}; [{cols}] or [{batch}, 1, .., {cols}] expected")
-    rows = p.reshape(-1, cols)
-    if rows.stride(1) != 1:
-        rows = rows.contiguous()
-    return rows, p.dim() > 1 and p.shape[0] == batch and batch > 1
+    dims = len(shape)
+    if dims == 0 or shape[-1] != cols or (dims > 1 and (shape[0] not in (1, batch) or
+                                                        any(n != 1 for n in shape[1:-1]))):
+        raise ValueError(f"{name}: shape {tuple(shape)}; [{cols}] or [{batch}, 1, .., {cols}] expected")
+    if p.stride(-1) != 1 and cols > 1:
+        p = p.contiguous()
+    return p, (p.data_ptr(), kind, p.stride(0) if dims > 1 and shape[0] == batch and batch > 1 else 0)
+
+
+_NO_PARAM = (None, 2, 0)
 
 
 class _Call:
-    """The checked arguments of a layer norm: x as ``[batch, rows, cols]`` and its parameters as rows."""
+    """The checked arguments of a layer norm: x as ``[batch, rows, cols]`` by its strides, and its parameters."""
+
+    __slots__ = ("x", "x_args", "cols", "eps", "device", "shape", "batch", "rows", "modulated", "params", "args", "keep")
 
     def __init__(self, x, weight, bias, scale, shift, eps):
-        if (weight is not None or bias is not None) and (scale is not None or shift is not None):
+        self.modulated = scale is not None or shift is not None
+        if self.modulated and (weight is not None or bias is not None):
             raise ValueError("layer_norm: weight and bias or scale and shift, not both")
         if not eps >= 0:
             raise ValueError(f"layer_norm: eps={eps}")
-        self.x_type = _lib.elem_type(x, "x")
-        if x.dim() == 0 or not 1 <= x.shape[-1] <= 16384:
-            raise ValueError(f"layer_norm: x of shape {tuple(x.shape)} (1..16384 columns)")
-        self.modulated = scale is not None or shift is not None
-        self.names = ("scale", "shift") if self.modulated else ("weight", "bias")
-        self.params = (scale, shift) if self.modulated else (weight, bias)
-        self.cols, self.eps, self.device, self.shape = x.shape[-1], float(eps), x.device, x.shape
-        batch = x.shape[0] if x.dim() > 1 else 1
-        (self.w, self.w_each), (self.b, self.b_each) = (
-            _param(p, self.cols, batch, x.device, n) for p, n in zip(self.params, self.names))
-        self.batch = batch if self.w_each or self.b_each else 1
-        self.x = self.rows_of(x)
-        self.rows = self.x.shape[1]
+        x_type = _lib.elem_type(x, "x")
+        self.shape = shape = x.shape
+        dims = len(shape)
+        if dims == 0 or not 1 <= shape[-1] <= 16384:
+            raise ValueError(f"layer_norm: x of shape {tuple(shape)} (1..16384 columns)")
+        self.x, self.cols, self.eps, self.device = x, shape[-1], eps, x.device
+        batch = shape[0] if dims > 1 else 1
+        if self.modulated:
+            self.params, names = (scale, shift), ("scale", "shift")
+        else:
+            self.params, names = (weight, bias), ("weight", "bias")
+        self.keep, self.args = [], []
+        for p, name in zip(self.params, names):
+            if p is None:
+                self.args.append(_NO_PARAM)
+            else:
+                p, args = _param(p, self.cols, batch, x.device, name)
+                self.keep.append(p)
+                self.args.append(args)
+        self.batch = batch if self.args[0][2] or self.args[1][2] else 1
+        self.rows = x.numel() // self.cols // self.batch if self.batch else 0
+        self.x_args = (*self.rows_of(x, x_type),)
 
-    def rows_of(self, t):
-        """A tensor of x's shape as ``[batch, rows, cols]`` with contiguous columns, in place where its strides allow."""
-        n = t.numel() // self.cols // self.batch if self.batch else 0
-        t = t.reshape(self.batch, n, self.cols)
-        return t if t.stride(2) == 1 else t.contiguous()
-
-    def param_args(self, p, each):
-        return (_lib.ptr(p), 2 if p is None else _lib.elem_type(p, ""), p.stride(0) if each else 0)
+    def rows_of(self, t, kind):
+        """A tensor of x's shape as the C entry takes it, ``(pointer, type, batch stride, row stride)``: in place where
+        its strides make rows of contiguous columns."""
+        if t.is_contiguous():
+            return t.data_ptr(), kind, self.rows * self.cols, self.cols
+        t = t.reshape(self.batch, self.rows, self.cols)
+        if t.stride(2) != 1 and self.cols > 1:
+            t = t.contiguous()
+        self.keep.append(t)
+        return t.data_ptr(), kind, t.stride(0), t.stride(1)
 
     def forward(self, y, y_type, q, s, fp8_type, mean, rstd):
-        _lib.launch(self.device, "svoo_layer_norm_fwd", self.x.data_ptr(), self.x_type, self.x.stride(0), self.x.stride(1),
-                    *self.param_args(self.w, self.w_each), *self.param_args(self.b, self.b_each), int(self.modulated),
-                    self.eps, self.batch, self.rows, self.cols, _lib.ptr(y), y_type, _lib.ptr(q), _lib.ptr(s), fp8_type,
-                    _lib.ptr(mean), _lib.ptr(rstd))
+        _lib.launch(self.device, "svoo_layer_norm_fwd", *self.x_args, *self.args[0], *self.args[1], self.modulated,
+                    self.eps, self.batch, self.rows, self.cols, y, y_type, q, s, fp8_type, mean, rstd)
 
 
-def _forward(c: _Call, x, out_dtype, stats: bool):
-    out_dtype = x.dtype if out_dtype is None else out_dtype
-    y = torch.empty(x.shape, dtype=out_dtype, device=x.device)
+def _forward(c: _Call, out_dtype, stats: bool):
+    """``(y, statistics [2, rows] or None)``."""
+    y = torch.empty(c.shape, dtype=out_dtype or c.x.dtype, device=c.device)
     y_type = _lib.elem_type(y, "out_dtype")
-    mean, rstd = (torch.empty(2, *x.shape[:-1], dtype=torch.float32, device=x.device) if stats else (None, None))
-    c.forward(y, y_type, None, None, 0, mean, rstd)
-    return y, mean, rstd
+    if not stats:
+        c.forward(y.data_ptr(), y_type, None, None, 0, None, None)
+        return y, None
+    rows = c.batch * c.rows
+    st = torch.empty((2, rows), dtype=torch.float32, device=c.device)
+    at = st.data_ptr()
+    c.forward(y.data_ptr(), y_type, None, None, 0, at, at + 4 * rows)
+    return y, st
 
 
 def layer_norm_fwd(x, weight=None, bias=None, *, scale=None, shift=None, eps=1e-6, out_dtype=None):
     """``(y, mean, rstd)`` of :func:`layer_norm`, with the fp32 statistics of every row (x's shape without its columns).
     No autograd."""
     _lib.refuse_grad("layer_norm_fwd", x, weight, bias, scale, shift)
-    return _forward(_Call(x, weight, bias, scale, shift, eps), x, out_dtype, True)
+    y, st = _forward(_Call(x, weight, bias, scale, shift, eps), out_dtype, True)
+    return y, st[0].view(x.shape[:-1]), st[1].view(x.shape[:-1])
 
 
 def layer_norm_bwd(dy, x, mean, rstd, weight=None, bias=None, *, scale=None, shift=None, eps=1e-6,
-                   needs: Tuple[bool, bool, bool] = (True, True, True)):
+                   needs: Sequence[bool] = (True, True, True)):
     """Gradients ``(dx, dweight, dbias)`` (``(dx, dscale, dshift)``) for the incoming ``dy``, from x and the statistics
     that :func:`layer_norm_fwd` returned.
 
     Pass the parameters the forward pass had: a gradient has its parameter's shape and type and is None without one, or
     where ``needs`` says so.  Sums over rows are fp32 in a fixed order: the same call gives the same bits."""
-    c = _Call(x, weight, bias, scale, shift, eps)
-    dy_type = _lib.elem_type(dy, "dy")
-    if dy.shape != x.shape or dy.device != x.device:
-        raise ValueError(f"dy: shape {tuple(dy.shape)} on {dy.device}, x {tuple(x.shape)} on {x.device}")
     for t, name in ((mean, "mean"), (rstd, "rstd")):
-        if t.dtype != torch.float32 or t.shape != x.shape[:-1] or t.device != x.device:
+        if not isinstance(t, torch.Tensor) or t.dtype != torch.float32 or t.shape != x.shape[:-1] or t.device != x.device:
             raise ValueError(f"{name}: fp32 of shape {tuple(x.shape[:-1])} on {x.device} expected")
     mean, rstd = mean.contiguous(), rstd.contiguous()
-    dy = c.rows_of(dy)
-    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if needs[0] else None
+    return _backward(dy, _Call(x, weight, bias, scale, shift, eps), mean.data_ptr(), rstd.data_ptr(), needs)
+
+
+def _backward(dy, c: _Call, mean: int, rstd: int, needs):
+    x = c.x
+    dy_type = _lib.elem_type(dy, "dy")
+    if dy.shape != c.shape or dy.device != c.device:
+        raise ValueError(f"dy: shape {tuple(dy.shape)} on {dy.device}, x {tuple(c.shape)} on {c.device}")
+    dy_args = c.rows_of(dy, dy_type)
+    dx = torch.empty(c.shape, dtype=x.dtype, device=c.device) if needs[0] else None
     want = [p is not None and need for p, need in zip(c.params, needs[1:])]
     if c.batch * c.rows == 0:
         return (dx, *(torch.zeros_like(p) if w else None for p, w in zip(c.params, want)))
     # a parameter shared by the batch entries of one that is not: its sums per entry, added here
-    grads = [None] * 2
-    for i, each in enumerate((c.w_each, c.b_each)):
+    grads = [None, None]
+    types = [2, 2]
+    for i, p in enumerate(c.params):
         if want[i]:
-            dtype = c.params[i].dtype if each or c.batch == 1 else torch.float32
-            grads[i] = torch.empty(c.batch, c.cols, dtype=dtype, device=x.device)
-    ws = None
-    if any(want):
-        ws = _lib.workspace(_lib.lib().svoo_layer_norm_bwd_workspace_size(c.batch, c.rows, c.cols), x.device)
-    types = [2 if g is None else _lib.elem_type(g, "") for g in grads]
-    _lib.launch(c.device, "svoo_layer_norm_bwd", c.x.data_ptr(), c.x_type, c.x.stride(0), c.x.stride(1), dy.data_ptr(),
-                dy_type, dy.stride(0), dy.stride(1), *c.param_args(c.w, c.w_each), int(c.modulated), mean.data_ptr(),
-                rstd.data_ptr(), c.batch, c.rows, c.cols, _lib.ptr(dx), _lib.ptr(grads[0]), types[0],
-                _lib.ptr(grads[1]), types[1], _lib.ptr(ws), ws.numel() if ws is not None else 0)
-    out = [None if g is None else (g if g.shape[0] == p.numel() // c.cols else g.sum(0)).to(p.dtype).view(p.shape)
-           for g, p in zip(grads, c.params)]
-    return (dx, *out)
+            own = c.args[i][2] or c.batch == 1
+            grads[i] = torch.empty(p.shape if own else (c.batch, c.cols), dtype=p.dtype if own else torch.float32,
+                                   device=c.device)
+            types[i] = _lib.elem_type(grads[i], "")
+    ws, size = None, 0
+    if want[0] or want[1]:
+        size = _lib.lib().svoo_layer_norm_bwd_workspace_size(c.batch, c.rows, c.cols)
+        if size:
+            ws = _lib.workspace(size, c.device)
+    _lib.launch(c.device, "svoo_layer_norm_bwd", *c.x_args, *dy_args, *c.args[0], c.modulated, mean, rstd, c.batch, c.rows,
+                c.cols, _lib.ptr(dx), _lib.ptr(grads[0]), types[0], _lib.ptr(grads[1]), types[1], _lib.ptr(ws), size)
+    for i, p in enumerate(c.params):
+        if grads[i] is not None and grads[i].shape != p.shape:
+            grads[i] = grads[i].sum(0).to(p.dtype).view(p.shape)
+    return dx, grads[0], grads[1]
 
 
 class _LayerNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, p0, p1, modulated, eps, out_dtype):
         params = (None, None, p0, p1) if modulated else (p0, p1, None, None)
-        y, mean, rstd = _forward(_Call(x, *params, eps), x, out_dtype, True)
-        ctx.save_for_backward(x, p0, p1, mean, rstd)
+        y, st = _forward(_Call(x, *params, eps), out_dtype, True)
+        ctx.save_for_backward(x, p0, p1, st)
         ctx.modulated, ctx.eps = modulated, eps
         return y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        x, p0, p1, mean, rstd = ctx.saved_tensors
-        kw = dict(scale=p0, shift=p1) if ctx.modulated else dict(weight=p0, bias=p1)
-        grads = layer_norm_bwd(dy, x, mean, rstd, eps=ctx.eps, needs=ctx.needs_input_grad[:3], **kw)
+        x, p0, p1, st = ctx.saved_tensors
+        params = (None, None, p0, p1) if ctx.modulated else (p0, p1, None, None)
+        at = st.data_ptr()
+        grads = _backward(dy, _Call(x, *params, ctx.eps), at, at + 4 * st.shape[1], ctx.needs_input_grad)
         return (*grads, None, None, None)
 
 
@@ -157,13 +186,12 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
     Parameters are ``[C]``, or ``[B, C]`` / ``[B, 1, .., C]`` with one row for each entry of x's first dimension
     (modulation vectors; strided ones are read in place).  Types may differ from x's.  The result has ``out_dtype``
     (x's by default).  Differentiable in x and the parameters, once."""
-    tensors = [t for t in (x, weight, bias, scale, shift) if t is not None]
-    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, scale, shift)):
         modulated = scale is not None or shift is not None
         if modulated and (weight is not None or bias is not None):
             raise ValueError("layer_norm: weight and bias or scale and shift, not both")
         return _LayerNorm.apply(x, scale if modulated else weight, shift if modulated else bias, modulated, eps, out_dtype)
-    return _forward(_Call(x, weight, bias, scale, shift, eps), x, out_dtype, False)[0]
+    return _forward(_Call(x, weight, bias, scale, shift, eps), out_dtype, False)[0]
 
 
 def layer_norm_fp8(x, weight=None, bias=None, *, scale=None, shift=None, eps=1e-6, dtype=torch.float8_e4m3fn):
@@ -174,5 +202,5 @@ def layer_norm_fp8(x, weight=None, bias=None, *, scale=None, shift=None, eps=1e-
         raise TypeError(f"layer_norm_fp8: float8_e4m3fn or float8_e5m2, got {dtype}")
     c = _Call(x, weight, bias, scale, shift, eps)
     q, s = empty_fp8(x.shape[:-1], c.cols, dtype, x.device), empty_scales(x.shape[:-1], c.cols, x.device)
-    c.forward(None, c.x_type, q, s, FP8_TYPES[dtype], None, None)
+    c.forward(None, c.x_args[1], q.data_ptr(), s.data_ptr(), FP8_TYPES[dtype], None, None)
     return q, s
