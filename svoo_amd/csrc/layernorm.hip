@@ -1,113 +1,54 @@
-// Layer norm, plain, affine or modulated per batch entry, with its backward pass.
-//   forward   n = (x - mean) rstd,  y = n w + b  (modulated: w = 1 + scale, b = shift of the row's batch entry)
-//   backward  g = dy w,  dx = rstd (g - mean(g) - n mean(g n)),  dw = sum_rows dy n,  db = sum_rows dy
-//
-// What bounds it: memory; forward reads x and writes y once, backward reads x and dy and writes dx once.  A row is held
-// in the registers of TPR lanes, eight consecutive elements per lane and chunk, so the mean and the centred second
-// moment are two passes over registers, not memory.  Lanes keep their columns from row to row: parameters are loaded
-// once per wave (twice the row's own bytes if loaded per row) and the column sums of the backward pass stay in
-// registers until the block's last row.  These go to one partial row per block and are added by a second kernel in a
-// fixed order, so gradients do not depend on the schedule.  Statistics, sums and gradients are fp32.
-#include <algorithm>
-#include <type_traits>
-
-#include "rows.h"
+// Layer norm: the forward pass, the C entries.
+#include "layernorm.h"
 
 namespace svoo {
 
-struct NormArgs {
-  const void* x;          // [batch][rows][cols], element strides
-  int x_type;
-  long long x_batch, x_row;
-  const void* w;          // weight or scale, [cols] per batch entry or null
-  const void* b;          // bias or shift or null
-  long long w_batch, b_batch;  // elements between batch entries (0: shared)
-  int w_type, b_type;
-  float w_plus;           // 1 for a scale
-  void* y;                // [batch * rows][cols] or null
-  int y_type;
-  uint8_t* q;             // 8-bit rows of padded columns or null
-  uint8_t* q_scale;
-  int fp8;
-  float* mean;            // [batch * rows] or null
-  float* rstd;
-  unsigned rows, rows_per_batch;
-  int cols;
-  float eps;
-};
-
-// Sums of a and b over the TPR lanes of a row, in each of them.  For rows of several waves every thread of the block
-// calls it; consecutive calls alternate between the two halves of scratch, so one barrier a call is enough.
-template <int TPR>
-__device__ __forceinline__ void row_sums(float& a, float& b, float2* scratch, int& half) {
-  if (TPR == 16) {
-    a = sum16(a);
-    b = sum16(b);
-  } else {
-    a = sum64(a);
-    b = sum64(b);
-    if (TPR > kWave) {
-      constexpr int kWaves = TPR / kWave;
-      float2* s = scratch + half * kWaves;
-      half ^= 1;
-      if (threadIdx.x % kWave == 0) s[threadIdx.x / kWave] = make_float2(a, b);
-      __syncthreads();
-      a = b = 0.0f;
-#pragma unroll
-      for (int i = 0; i < kWaves; ++i) {
-        a += s[i].x;
-        b += s[i].y;
-      }
-    }
-  }
-}
-
-template <int TPR, int NC, bool kWhole>
-__device__ __forceinline__ void load_params(const void* p, int type, long long at, float plus, float none, int cols, int t,
-                                            float (&v)[NC][8]) {
-  if (p != nullptr) load_row<TPR, NC, kWhole>(p, type, at, cols, t, v);
-#pragma unroll
-  for (int c = 0; c < NC; ++c)
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[c][e] = p != nullptr ? v[c][e] + plus : none;
-}
-
-template <int TPR, int NC, bool kWhole, bool kFp8>
-__global__ void __launch_bounds__(TPR > 256 ? TPR : 256) norm_fwd_kernel(NormArgs a) {
-  constexpr int kThreads = TPR > 256 ? TPR : 256, kGroups = kThreads / TPR;
-  __shared__ float2 scratch[2 * (TPR > kWave ? TPR / kWave : 1)];
-  int half = 0;
-  const int t = threadIdx.x % TPR, group = threadIdx.x / TPR;
+// What bounds it: memory.  16 lanes hold a row of up to 128 columns, a wave one of up to 10 chunks of 512, a block of 1024
+// threads a wider one, as it lies in memory: the mean and the centred second moment are two passes over registers, and
+// with 46 of them at 1536 columns eight waves a SIMD keep enough loads in flight.  A block's rows share a batch entry,
+// whose parameters lie in LDS: in registers they would take more than the row, and loaded per row twice its bytes.
+// Measured, modulated bf16: 32760 x 1536 36 us (5.6 TB/s; 66 us with parameters and the row's values in fp32 registers),
+// 75600 x 5120 310 us (5.0 TB/s; 777 us).  Over widths of 128 to 8192 in whole chunks 4.0 to 5.2 TB/s, a wave per row
+// 20% above a block of 256 per row at 5120; rows of an odd length above 1536 columns, element by element at the end and
+// with no chunk on a 16-byte address, 1.8 to 3.3 TB/s.
+template <int T, int TPR, int NC, bool kWhole, bool kFp8>
+__device__ __forceinline__ void norm_rows(const NormArgs& a, const f32x4_t* w, const f32x4_t* b, float2* scratch) {
+  const int groups = blockDim.x / TPR, t = threadIdx.x % TPR;
+  const unsigned batch = blockIdx.x / a.parts, part = blockIdx.x % a.parts;
   const float inv = 1.0f / (float)a.cols;
-  float w[NC][8], b[NC][8];
-  unsigned loaded = ~0u;
-  for (unsigned row = blockIdx.x * kGroups + group; row < a.rows; row += gridDim.x * kGroups) {
-    const unsigned batch = row / a.rows_per_batch;
-    const long long at = batch * a.x_batch + (row - batch * a.rows_per_batch) * a.x_row;
-    float x[NC][8];
-    load_row<TPR, NC, kWhole>(a.x, a.x_type, at, a.cols, t, x);
-    if (loaded != batch) {
-      load_params<TPR, NC, kWhole>(a.w, a.w_type, batch * a.w_batch, a.w_plus, 1.0f, a.cols, t, w);
-      load_params<TPR, NC, kWhole>(a.b, a.b_type, batch * a.b_batch, 0.0f, 0.0f, a.cols, t, b);
-      loaded = batch;
-    }
-    float s = 0.0f, unused = 0.0f;
+  int half = 0;
+  for (unsigned r = part * groups + threadIdx.x / TPR; r < a.rows_per_batch; r += a.parts * groups) {
+    const size_t row = (size_t)batch * a.rows_per_batch + r;
+    RawRow<T, NC> x;
+    x.template load<TPR, kWhole>(a.x, batch * a.x_batch + r * a.x_row, a.cols, t);
+    float s0 = 0.0f, s1 = 0.0f;
 #pragma unroll
     for (int c = 0; c < NC; ++c)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) s += x[c][e];
-    row_sums<TPR>(s, unused, scratch, half);
-    const float mean0 = s * inv;
+      for (int e = 0; e < 8; e += 2) {
+        s0 += x.at(c, e);
+        s1 += x.at(c, e + 1);
+      }
+    s0 += s1;
+    s1 = 0.0f;
+    row_sums<TPR>(s0, s1, scratch, half);
+    float mean0 = s0 * inv;
+    __asm__("" : "+v"(mean0));  // rounded once: fused into some of the differences below it would not be the same in all
+    x.forget();
     float d1 = 0.0f, d2 = 0.0f;
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
       const int col = (c * TPR + t) * 8;
+      float u1 = 0.0f, u2 = 0.0f;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        x[c][e] = col + (kWhole ? 0 : e) < a.cols ? x[c][e] - mean0 : 0.0f;
-        d1 += x[c][e];
-        d2 = fmaf(x[c][e], x[c][e], d2);
+        const float d = kWhole || col + e < a.cols ? x.at(c, e) - mean0 : 0.0f;
+        u1 += d;
+        u2 = fmaf(d, d, u2);
       }
+      const bool in = !kWhole || col < a.cols;
+      d1 += in ? u1 : 0.0f;
+      d2 += in ? u2 : 0.0f;
     }
     row_sums<TPR>(d1, d2, scratch, half);
     // what the rounding of the mean left over: the deviations' own mean
@@ -116,27 +57,31 @@ __global__ void __launch_bounds__(TPR > 256 ? TPR : 256) norm_fwd_kernel(NormArg
       if (a.mean != nullptr) a.mean[row] = mean0 + dm;
       if (a.rstd != nullptr) a.rstd[row] = rstd;
     }
+    x.forget();
+    const int blocks = (a.cols + 127) / 128;
 #pragma unroll
-    for (int c = 0; c < NC; ++c)
+    for (int c = 0; c < NC; ++c) {
+      const int col = (c * TPR + t) * 8;
+      float y[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) x[c][e] = fmaf((x[c][e] - dm) * rstd, w[c][e], b[c][e]);
-    if (!kFp8) {
-      store_row<TPR, NC, kWhole>(a.y, a.y_type, (long long)row * a.cols, a.cols, t, x);
-    } else {
-      const int blocks = (a.cols + 127) / 128;
+      for (int h = 0; h < 2; ++h) {
+        const f32x4_t wv = w[(c * 2 + h) * TPR + t], bv = b[(c * 2 + h) * TPR + t];
 #pragma unroll
-      for (int c = 0; c < NC; ++c) {
-        const int col = (c * TPR + t) * 8;
+        for (int e = 0; e < 4; ++e) y[4 * h + e] = fmaf((x.at(c, 4 * h + e) - mean0 - dm) * rstd, wv[e], bv[e]);
+      }
+      if (!kFp8) {
+        store_row8_as<kWhole>(a.y, a.y_type, (long long)row * a.cols + col, a.cols - col, y);
+      } else {
         // the rounded row, as a quantiser of the stored one would see it; 16 lanes hold a block of 128 columns
         float amax = 0.0f;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          x[c][e] = col + (kWhole ? 0 : e) < a.cols ? row_round(a.y_type, x[c][e]) : 0.0f;
-          amax = fmaxf(amax, finite_abs(x[c][e]));
+          y[e] = col + (kWhole ? 0 : e) < a.cols ? row_round(a.y_type, y[e]) : 0.0f;
+          amax = fmaxf(amax, finite_abs(y[e]));
         }
         const int e8 = block_exponent(max16(amax), a.fp8);
         if (col < blocks * 128) {
-          *(uint2*)(a.q + (size_t)row * blocks * 128 + col) = quantize8(x[c], e8, a.fp8);
+          *(uint2*)(a.q + (size_t)row * blocks * 128 + col) = quantize8(y, e8, a.fp8);
           if (t % 16 == 0) a.q_scale[(size_t)(col / 128) * a.rows + row] = (uint8_t)(e8 + 127);
         }
       }
@@ -144,99 +89,19 @@ __global__ void __launch_bounds__(TPR > 256 ? TPR : 256) norm_fwd_kernel(NormArg
   }
 }
 
-struct NormGradArgs {
-  const void* x;
-  int x_type;
-  long long x_batch, x_row;
-  const void* dy;          // element strides
-  long long dy_batch, dy_row;
-  int dy_type;
-  const void* w;
-  long long w_batch;
-  int w_type;
-  float w_plus;
-  const float* mean;
-  const float* rstd;
-  void* dx;                // [batch * rows][cols], type of x, or null
-  float* partial;          // [batch][parts][2][cols] or null (no parameter gradients)
-  void* dw;                // with one part the sums go straight to the gradients
-  void* db;
-  int dw_type, db_type;
-  unsigned rows_per_batch, parts;
-  int cols;
-};
-
-template <int TPR, int NC, bool kWhole>
-__global__ void __launch_bounds__(TPR > 256 ? TPR : 256) norm_bwd_kernel(NormGradArgs a) {
-  constexpr int kThreads = TPR > 256 ? TPR : 256, kGroups = kThreads / TPR;
+template <int T, int TPR, int NC, bool kWhole, bool kFp8>
+__global__ void __launch_bounds__(TPR > 256 ? TPR : 256) norm_fwd_kernel(NormArgs a) {
+  __shared__ f32x4_t params[2][2 * NC * TPR];  // four columns each: chunk, half, lane
   __shared__ float2 scratch[2 * (TPR > kWave ? TPR / kWave : 1)];
-  __shared__ float sums[kGroups > 1 ? (kGroups - 1) * TPR * 8 : 1];
-  int half = 0;
-  const int t = threadIdx.x % TPR, group = threadIdx.x / TPR;
-  const unsigned batch = blockIdx.x / a.parts, part = blockIdx.x % a.parts;
-  const float inv = 1.0f / (float)a.cols;
-  float w[NC][8], dw[NC][8], db[NC][8];
-  load_params<TPR, NC, kWhole>(a.w, a.w_type, batch * a.w_batch, a.w_plus, 1.0f, a.cols, t, w);
-#pragma unroll
-  for (int c = 0; c < NC; ++c)
-#pragma unroll
-    for (int e = 0; e < 8; ++e) dw[c][e] = db[c][e] = 0.0f;
-  for (unsigned r = part * kGroups + group; r < a.rows_per_batch; r += a.parts * kGroups) {
-    const size_t row = (size_t)batch * a.rows_per_batch + r;
-    const float mean = a.mean[row], rstd = a.rstd[row];
-    float n[NC][8], g[NC][8];
-    float s1 = 0.0f, s2 = 0.0f;
-    load_row<TPR, NC, kWhole>(a.x, a.x_type, batch * a.x_batch + r * a.x_row, a.cols, t, n);
-    load_row<TPR, NC, kWhole>(a.dy, a.dy_type, batch * a.dy_batch + r * a.dy_row, a.cols, t, g);
-#pragma unroll
-    for (int c = 0; c < NC; ++c)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        n[c][e] = (n[c][e] - mean) * rstd;  // past the row's end dy is 0, and so is whatever n enters
-        db[c][e] += g[c][e];
-        dw[c][e] = fmaf(g[c][e], n[c][e], dw[c][e]);
-        g[c][e] *= w[c][e];
-        s1 += g[c][e];
-        s2 = fmaf(g[c][e], n[c][e], s2);
-      }
-    if (a.dx == nullptr) continue;
-    row_sums<TPR>(s1, s2, scratch, half);
-    s1 *= inv;
-    s2 *= inv;
-#pragma unroll
-    for (int c = 0; c < NC; ++c)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) g[c][e] = rstd * (g[c][e] - s1 - n[c][e] * s2);
-    store_row<TPR, NC, kWhole>(a.dx, a.x_type, (long long)row * a.cols, a.cols, t, g);
+  const unsigned batch = blockIdx.x / a.parts;
+  for (int i = threadIdx.x; i < NC * TPR * 8; i += blockDim.x) {
+    const int at = ((i / (TPR * 8) * 2 + i / 4 % 2) * TPR + i / 8 % TPR) * 4 + i % 4;
+    const bool in = i < a.cols;
+    ((float*)params[0])[at] = in && a.w != nullptr ? row_elem(a.w, a.w_type, batch * a.w_batch + i) + a.w_plus : 1.0f;
+    ((float*)params[1])[at] = in && a.b != nullptr ? row_elem(a.b, a.b_type, batch * a.b_batch + i) : 0.0f;
   }
-  if (a.partial == nullptr && a.dw == nullptr && a.db == nullptr) return;
-#pragma unroll
-  for (int which = 0; which < 2; ++which) {
-    float v[NC][8];
-#pragma unroll
-    for (int c = 0; c < NC; ++c) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[c][e] = which == 0 ? dw[c][e] : db[c][e];
-      if (kGroups > 1) {  // the block's groups, in their order
-        __syncthreads();
-        if (group > 0)
-#pragma unroll
-          for (int e = 0; e < 8; ++e) sums[((group - 1) * 8 + e) * TPR + t] = v[c][e];
-        __syncthreads();
-        if (group == 0)
-          for (int k = 0; k < kGroups - 1; ++k)
-#pragma unroll
-            for (int e = 0; e < 8; ++e) v[c][e] += sums[(k * 8 + e) * TPR + t];
-      }
-    }
-    if (group != 0) continue;
-    if (a.partial != nullptr)
-      store_row<TPR, NC, kWhole>(a.partial, kRowF32, ((long long)blockIdx.x * 2 + which) * a.cols, a.cols, t, v);
-    else if (which == 0 && a.dw != nullptr)
-      store_row<TPR, NC, kWhole>(a.dw, a.dw_type, (long long)batch * a.cols, a.cols, t, v);
-    else if (which == 1 && a.db != nullptr)
-      store_row<TPR, NC, kWhole>(a.db, a.db_type, (long long)batch * a.cols, a.cols, t, v);
-  }
+  __syncthreads();
+  norm_rows<T, TPR, NC, kWhole, kFp8>(a, params[0], params[1], scratch);
 }
 
 // out[batch][col] = sum over parts of partial[batch][part][which][col]: 64 columns a block, 16 slices of the parts.
@@ -261,31 +126,31 @@ __global__ void __launch_bounds__(1024) norm_param_grad_kernel(const float* __re
   set_row_elem(out, which == 0 ? dw_type : db_type, (long long)blockIdx.z * cols + col, s);
 }
 
-// Lanes per row and chunks of eight elements a lane, from the row's width: rows up to 1536 columns fit one wave's
-// registers (three chunks with their parameters and column sums, three waves per SIMD), wider ones a block.
+// Lanes per row and chunks of eight elements a lane, from the row's width; fewer classes for the slower rows that do not
+// end with a chunk.
 template <class F>
 static void for_width(int cols, F f) {
+  const bool whole = cols % 8 == 0;
   if (cols <= 128) f(std::integral_constant<int, 16>(), std::integral_constant<int, 1>());
   else if (cols <= 512) f(std::integral_constant<int, 64>(), std::integral_constant<int, 1>());
-  else if (cols <= 1024) f(std::integral_constant<int, 64>(), std::integral_constant<int, 2>());
+  else if (whole && cols <= 1024) f(std::integral_constant<int, 64>(), std::integral_constant<int, 2>());
   else if (cols <= 1536) f(std::integral_constant<int, 64>(), std::integral_constant<int, 3>());
-  else if (cols <= 2048) f(std::integral_constant<int, 256>(), std::integral_constant<int, 1>());
-  else if (cols <= 4096) f(std::integral_constant<int, 256>(), std::integral_constant<int, 2>());
-  else if (cols <= 6144) f(std::integral_constant<int, 256>(), std::integral_constant<int, 3>());
+  else if (whole && cols <= 2560) f(std::integral_constant<int, 64>(), std::integral_constant<int, 5>());
+  else if (whole && cols <= 5120) f(std::integral_constant<int, 64>(), std::integral_constant<int, 10>());
   else if (cols <= 8192) f(std::integral_constant<int, 1024>(), std::integral_constant<int, 1>());
   else f(std::integral_constant<int, 1024>(), std::integral_constant<int, 2>());
 }
 template <class F>
-static void for_flag(bool v, F f) {
-  if (v) f(std::true_type());
-  else f(std::false_type());
+static void for_type(int type, F f) {
+  if (type == kRowBf16) f(std::integral_constant<int, kRowBf16>());
+  else if (type == kRowF16) f(std::integral_constant<int, kRowF16>());
+  else f(std::integral_constant<int, kRowF32>());
 }
 
-static int groups_for(int cols) { return cols <= 128 ? 16 : cols <= 1536 ? 4 : 1; }
-
-// Blocks that share a batch entry's rows: two per CU in all, and no fewer than four rows a group where there are more.
+// Blocks that share a batch entry's rows in the backward pass: two per CU in all, and no fewer than four rows a group
+// where there are more.
 static unsigned grad_parts(long long batch, long long rows_per_batch, int cols) {
-  const long long groups = groups_for(cols);
+  const long long groups = cols <= 128 ? 16 : cols <= 1536 ? 4 : 1;
   const long long most = std::max(512 / batch, 1ll), want = (rows_per_batch + 4 * groups - 1) / (4 * groups);
   return (unsigned)std::min(most, std::max(want, 1ll));
 }
@@ -322,17 +187,25 @@ extern "C" int svoo_layer_norm_fwd(const void* x, int x_type, long long x_batch_
                "%s: one of y and (q, q_scale)", name);
   SVOO_REQUIRE((uintptr_t)q % 8 == 0, SVOO_ERR_INVALID_ARG, "%s: q must start at an 8-byte address", name);
   SVOO_REQUIRE(x, SVOO_ERR_INVALID_ARG, "%s: null pointer", name);
-  const NormArgs a = {x,      x_type, x_batch_stride, x_row_stride, w,      b,  w_batch_stride, b_batch_stride, w_type,
-                      b_type, modulated ? 1.0f : 0.0f, y,   y_type, q,  q_scale,        fp8_type,       mean,
-                      rstd,   (unsigned)rows, (unsigned)rows_per_batch, cols, eps};
+  NormArgs a = {x, x_type, x_batch_stride, x_row_stride, w, b, w_batch_stride, b_batch_stride, w_type, b_type,
+                modulated ? 1.0f : 0.0f, y, y_type, q, q_scale, fp8_type, mean, rstd, (unsigned)rows,
+                (unsigned)rows_per_batch, 1, cols, eps};
   for_width(cols, [&](auto tpr, auto nc) {
-    constexpr int kTpr = decltype(tpr)::value, kNc = decltype(nc)::value, kThreads = kTpr > 256 ? kTpr : 256;
-    const long long groups = kThreads / kTpr, cap = kTpr > 256 ? 512 : 2048;
-    const dim3 grid((unsigned)std::min((rows + groups - 1) / groups, cap)), block(kThreads);
-    for_flag(cols % 8 == 0, [&](auto whole) {
-      for_flag(q != nullptr, [&](auto to_fp8) {
-        hipLaunchKernelGGL((norm_fwd_kernel<kTpr, kNc, decltype(whole)::value, decltype(to_fp8)::value>), grid, block, 0,
-                           (hipStream_t)stream, a);
+    constexpr int kTpr = decltype(tpr)::value, kNc = decltype(nc)::value;
+    constexpr int kThreads = kTpr > 256 ? kTpr : 256;
+    // blocks that are resident (32 waves a CU at most), the rest of the rows in turn
+    const long long groups = kThreads / kTpr, want = (rows_per_batch + groups - 1) / groups;
+    a.parts = (unsigned)std::min(want, std::max(256 * (2048 / kThreads) / batch, 1ll));
+    const dim3 grid((unsigned)(batch * a.parts)), block(kThreads);
+    for_type(x_type, [&](auto type) {
+      for_flag(cols % 8 == 0, [&](auto whole) {
+        constexpr bool kWhole = decltype(whole)::value;
+        if constexpr (kWhole || kNc == 1 || kNc == 3 || kTpr == 1024) {
+          for_flag(q != nullptr, [&](auto to_fp8) {
+            hipLaunchKernelGGL((norm_fwd_kernel<decltype(type)::value, kTpr, kNc, kWhole, decltype(to_fp8)::value>), grid,
+                               block, 0, (hipStream_t)stream, a);
+          });
+        }
       });
     });
   });
@@ -363,23 +236,16 @@ extern "C" int svoo_layer_norm_bwd(const void* x, int x_type, long long x_batch_
   }
   SVOO_REQUIRE(x && dy && mean && rstd, SVOO_ERR_INVALID_ARG, "%s: null pointer", name);
   if (!dx && !dw && !db) return SVOO_OK;
-  const bool params = dw || db;
   const unsigned parts = grad_parts(batch, rows_per_batch, cols);
-  const bool joined = params && parts > 1;
+  const bool joined = (dw || db) && parts > 1;
   SVOO_REQUIRE(!joined || (workspace && ws_bytes >= svoo_layer_norm_bwd_workspace_size(batch, rows_per_batch, cols)),
                SVOO_ERR_WORKSPACE, "%s: workspace of %zu bytes (%zu needed)", name, ws_bytes,
                svoo_layer_norm_bwd_workspace_size(batch, rows_per_batch, cols));
-  const NormGradArgs a = {x,       x_type, x_batch_stride, x_row_stride, dy,   dy_batch_stride, dy_row_stride,
-                          dy_type, w,              w_batch_stride, w_type, modulated ? 1.0f : 0.0f, mean,
-                          rstd,    dx,             joined ? (float*)workspace : nullptr, joined ? nullptr : dw,
-                          joined ? nullptr : db, dw_type, db_type, (unsigned)rows_per_batch, parts, cols};
-  for_width(cols, [&](auto tpr, auto nc) {
-    constexpr int kTpr = decltype(tpr)::value, kNc = decltype(nc)::value, kThreads = kTpr > 256 ? kTpr : 256;
-    for_flag(cols % 8 == 0, [&](auto whole) {
-      hipLaunchKernelGGL((norm_bwd_kernel<kTpr, kNc, decltype(whole)::value>), dim3((unsigned)(batch * parts)),
-                         dim3(kThreads), 0, (hipStream_t)stream, a);
-    });
-  });
+  const NormGradArgs a = {x, x_type, x_batch_stride, x_row_stride, dy, dy_type, dy_batch_stride, dy_row_stride, w,
+                          w_batch_stride, w_type, modulated ? 1.0f : 0.0f, mean, rstd, dx,
+                          joined ? (float*)workspace : nullptr, joined ? nullptr : dw, joined ? nullptr : db, dw_type,
+                          db_type, (unsigned)rows_per_batch, parts, cols};
+  launch_norm_bwd(a, batch, (hipStream_t)stream);
   if (const int rc = check_launch(name)) return rc;
   if (!joined) return SVOO_OK;
   hipLaunchKernelGGL(norm_param_grad_kernel, dim3((cols + kWave - 1) / kWave, 2, (unsigned)batch), dim3(1024), 0,

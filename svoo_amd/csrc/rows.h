@@ -86,33 +86,59 @@ __device__ __forceinline__ void store_row8(void* p, long long i, int n, const fl
   }
 }
 
-// A row's share of lane t of TPR: NC chunks of eight elements, (c TPR + t) 8 .. + 7 of cols.  The type is uniform, so its
-// branch is outside the loop and a row's loads leave together.
-template <int TPR, int NC, bool kWhole>
-__device__ __forceinline__ void load_row(const void* p, int type, long long at, int cols, int t, float (&v)[NC][8]) {
-  if (type == kRowBf16) {
+// A row's share of lane t of TPR as it lies in memory: NC chunks of eight elements, (c TPR + t) 8 .. + 7 of cols, zeros
+// past the end.  Half as many registers as its values in fp32 take; they are converted where they are used.
+template <int T, int NC>
+struct RawRow {
+  u32x4_t v[NC][T == kRowF32 ? 2 : 1];
+
+  template <int TPR, bool kWhole>
+  __device__ __forceinline__ void load(const void* p, long long at, int cols, int t) {
 #pragma unroll
-    for (int c = 0; c < NC; ++c) load_row8<kRowBf16, kWhole>(p, at + (c * TPR + t) * 8, cols - (c * TPR + t) * 8, v[c]);
-  } else if (type == kRowF16) {
+    for (int c = 0; c < NC; ++c) {
+      const int n = cols - (c * TPR + t) * 8;
+      const long long i = at + (c * TPR + t) * 8;
+      if (n >= 8) {
+        if (T == kRowF32) {
+          v[c][0] = ((const Dwords4*)((const float*)p + i))->v;
+          v[c][T == kRowF32 ? 1 : 0] = ((const Dwords4*)((const float*)p + i + 4))->v;
+        } else {
+          v[c][0] = ((const Dwords4*)((const uint16_t*)p + i))->v;
+        }
+      } else {
 #pragma unroll
-    for (int c = 0; c < NC; ++c) load_row8<kRowF16, kWhole>(p, at + (c * TPR + t) * 8, cols - (c * TPR + t) * 8, v[c]);
-  } else {
+        for (int h = 0; h < (T == kRowF32 ? 2 : 1); ++h) v[c][h] = u32x4_t{0, 0, 0, 0};
+        if (!kWhole) {
 #pragma unroll
-    for (int c = 0; c < NC; ++c) load_row8<kRowF32, kWhole>(p, at + (c * TPR + t) * 8, cols - (c * TPR + t) * 8, v[c]);
+          for (int e = 0; e < 8; ++e)
+            if (e < n) {
+              if (T == kRowF32) v[c][T == kRowF32 ? e / 4 : 0][e % 4] = ((const uint32_t*)p)[i + e];
+              else v[c][0][e / 2] |= (uint32_t)((const uint16_t*)p)[i + e] << (16 * (e & 1));
+            }
+        }
+      }
+    }
   }
-}
-template <int TPR, int NC, bool kWhole>
-__device__ __forceinline__ void store_row(void* p, int type, long long at, int cols, int t, const float (&v)[NC][8]) {
-  if (type == kRowBf16) {
+  // Values converted before are converted again: held in fp32 they would take the registers that this type saves.
+  __device__ __forceinline__ void forget() {
 #pragma unroll
-    for (int c = 0; c < NC; ++c) store_row8<kRowBf16, kWhole>(p, at + (c * TPR + t) * 8, cols - (c * TPR + t) * 8, v[c]);
-  } else if (type == kRowF16) {
+    for (int c = 0; c < NC; ++c)
 #pragma unroll
-    for (int c = 0; c < NC; ++c) store_row8<kRowF16, kWhole>(p, at + (c * TPR + t) * 8, cols - (c * TPR + t) * 8, v[c]);
-  } else {
-#pragma unroll
-    for (int c = 0; c < NC; ++c) store_row8<kRowF32, kWhole>(p, at + (c * TPR + t) * 8, cols - (c * TPR + t) * 8, v[c]);
+      for (int h = 0; h < (T == kRowF32 ? 2 : 1); ++h) __asm__ volatile("" : "+v"(v[c][h]));
   }
+  __device__ __forceinline__ float at(int c, int e) const {
+    if (T == kRowF32) return __uint_as_float(v[c][T == kRowF32 ? e / 4 : 0][e % 4]);
+    if (T == kRowBf16) return __uint_as_float(e & 1 ? v[c][0][e / 2] & 0xffff0000u : v[c][0][e / 2] << 16);
+    return (float)__builtin_bit_cast(_Float16, (uint16_t)(v[c][0][e / 2] >> (16 * (e & 1))));
+  }
+};
+
+// Eight values of a row's share to memory, by the (uniform) type.
+template <bool kWhole>
+__device__ __forceinline__ void store_row8_as(void* p, int type, long long i, int n, const float (&f)[8]) {
+  if (type == kRowBf16) store_row8<kRowBf16, kWhole>(p, i, n, f);
+  else if (type == kRowF16) store_row8<kRowF16, kWhole>(p, i, n, f);
+  else store_row8<kRowF32, kWhole>(p, i, n, f);
 }
 
 // ---------------------------------------------------------------- sums and maxima over lanes, in every lane
@@ -136,6 +162,27 @@ __device__ __forceinline__ float sum64(float v) {
   v = sum16(v);
   const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
   return xhalf_sum(__uint_as_float(r[0]) + __uint_as_float(r[1]));
+}
+
+// Sums of a and b over the TPR lanes of a row, in each of them.  For rows of several waves every thread of the block
+// calls it; consecutive calls alternate between the two halves of scratch, so one barrier a call is enough.
+template <int TPR>
+__device__ __forceinline__ void row_sums(float& a, float& b, float2* scratch, int& half) {
+  a = TPR == 16 ? sum16(a) : sum64(a);
+  b = TPR == 16 ? sum16(b) : sum64(b);
+  if (TPR > kWave) {
+    constexpr int kWaves = TPR / kWave;
+    float2* s = scratch + half * kWaves;
+    half ^= 1;
+    if (threadIdx.x % kWave == 0) s[threadIdx.x / kWave] = make_float2(a, b);
+    __syncthreads();
+    a = b = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kWaves; ++i) {
+      a += s[i].x;
+      b += s[i].y;
+    }
+  }
 }
 
 // ---------------------------------------------------------------- 8-bit blocks
