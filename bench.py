@@ -51,6 +51,8 @@ def parse_args():
     ap.add_argument("--pattern", default="SAP", choices=["SAP", "EAR"],
                     help="SAP: top-p block mask (the headline); EAR: error-aware routing with centroid compensation "
                          "(Wan configs)")
+    ap.add_argument("--linear", default="bf16", choices=["bf16", "fp8"],
+                    help="C5: fp8 puts 8-bit linear layers and fused norms into the DiT's blocks")
     ap.add_argument("--sparsity-profile", action="store_true",
                     help="time the offline profile producer (exact per-head sparsity of one layer) instead")
     ap.add_argument("--no-dense", action="store_true", help="skip the dense SDPA comparator")
@@ -512,7 +514,7 @@ def main_dit(args):
     import torch
 
     from svoo_amd import _lib, dit
-    from svoo_amd.inference import replace_wan_attention
+    from svoo_amd.inference import replace_wan_attention, replace_wan_linear
     from svoo_amd.processor import WanAttn_SAPAttn_Processor
 
     if not torch.cuda.is_available():
@@ -556,6 +558,9 @@ def main_dit(args):
                 num_k_centroids=1024, top_p_kmeans=top_p, min_kc_ratio=0.10, kmeans_iter_init=2, kmeans_iter_step=2,
                 start_reuse_step=None, reuse_interval=1, use_dynamic_min_kc_ratio=True, sparsity_csv_path=str(csv),
                 dynamic_min_kc_ratio_min=dmin, dynamic_min_kc_ratio_max=dmax, processor_cls=Proc)
+    if args.linear == "fp8":
+        replace_wan_linear(pipe)
+        model.fuse_norms()
     n = Proc.num_frame * Proc.frame_size
     assert n == 32760, n
     timesteps = iter(np.linspace(999.0, 600.0, 10 * nsteps))
@@ -621,7 +626,7 @@ def main_dit(args):
         log(f"dense step {t_dense:.2f} ms")
 
     cpu = None
-    if not args.no_cpu:
+    if not args.no_cpu and args.linear == "bf16":  # the sample runs the blocks' own 16-bit projections
         cpu = cpu_baseline_dit(model, lat, txt, rho, top_p, dmin, dmax, args.cpu_heads, t_step, dev)
 
     line = {
@@ -635,7 +640,7 @@ def main_dit(args):
         "higher_is_better": False,
         "scaling": "weak",
         "vs_baseline": None,
-        "dtype": "bf16",
+        "dtype": "bf16" if args.linear == "bf16" else "bf16; e4m3 operands in the blocks' linear layers",
         "data": "synthetic (random-init weights, Gaussian latents and text embeddings, U[0.05,0.4] profile)",
         "config": {
             "workload": f"C5-wan2.1-1.3B-dit-step: 30 blocks, dim 1536, 12 heads, FFN 8960, N={n}, 512 text tokens, "

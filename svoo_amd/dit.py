@@ -20,6 +20,9 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
+from . import norm
+from .fp8 import Fp8Linear
+
 
 @dataclass
 class WanDiTConfig:
@@ -48,9 +51,13 @@ class DenseWanAttnProcessor:
     def __call__(self, attn, hidden_states, encoder_hidden_states=None, attention_mask=None, rotary_emb=None,
                  timestep=None):
         ctx = hidden_states if encoder_hidden_states is None else encoder_hidden_states
-        q = attn.norm_q(attn.to_q(hidden_states)).unflatten(2, (attn.heads, -1))
-        k = attn.norm_k(attn.to_k(ctx)).unflatten(2, (attn.heads, -1))
-        v = attn.to_v(ctx).unflatten(2, (attn.heads, -1))
+        if encoder_hidden_states is None and getattr(attn, "fused_projections", False):
+            q, k, v = attn.to_qkv(hidden_states).chunk(3, dim=-1)
+        else:
+            q, k, v = attn.to_q(hidden_states), attn.to_k(ctx), attn.to_v(ctx)
+        q = attn.norm_q(q).unflatten(2, (attn.heads, -1))
+        k = attn.norm_k(k).unflatten(2, (attn.heads, -1))
+        v = v.unflatten(2, (attn.heads, -1))
         if rotary_emb is not None:
             q = apply_rope(q, *rotary_emb)
             k = apply_rope(k, *rotary_emb)
@@ -102,7 +109,12 @@ class WanAttention(nn.Module):
 
 
 class WanBlock(nn.Module):
-    """One Wan DiT block: modulated self-attention, cross-attention to the text, modulated FFN."""
+    """One Wan DiT block: modulated self-attention, cross-attention to the text, modulated FFN.
+
+    With ``fused_norms`` each norm and its modulation are one pass (:func:`svoo_amd.norm.layer_norm`, differentiable),
+    and an 8-bit FFN (:func:`svoo_amd.inference.replace_wan_linear`) takes its input as 8-bit rows from the norm."""
+
+    fused_norms = False
 
     def __init__(self, cfg: WanDiTConfig):
         super().__init__()
@@ -120,13 +132,25 @@ class WanBlock(nn.Module):
         mod = (self.scale_shift_table.float() + temb.float()).chunk(6, dim=1)
         shift, scale, gate, c_shift, c_scale, c_gate = mod
         dtype = hidden_states.dtype
-        x = (self.norm1(hidden_states.float()) * (1 + scale) + shift).to(dtype)
+        if self.fused_norms:
+            x = norm.layer_norm(hidden_states, scale=scale, shift=shift, eps=self.norm1.eps)
+        else:
+            x = (self.norm1(hidden_states.float()) * (1 + scale) + shift).to(dtype)
         a = self.attn1(hidden_states=x, rotary_emb=rotary_emb, timestep=timestep)
         hidden_states = (hidden_states.float() + a.float() * gate).to(dtype)
-        x = self.norm2(hidden_states.float()).to(dtype)
+        if self.fused_norms:
+            x = norm.layer_norm(hidden_states, self.norm2.weight, self.norm2.bias, eps=self.norm2.eps)
+        else:
+            x = self.norm2(hidden_states.float()).to(dtype)
         hidden_states = hidden_states + self.attn2(hidden_states=x, encoder_hidden_states=encoder_hidden_states)
-        x = (self.norm3(hidden_states.float()) * (1 + c_scale) + c_shift).to(dtype)
-        f = self.ffn(x)
+        if self.fused_norms and isinstance(self.ffn[0], Fp8Linear):
+            rows = norm.layer_norm_fp8(hidden_states, scale=c_scale, shift=c_shift, eps=self.norm3.eps)
+            f = self.ffn[1:](self.ffn[0].forward_quantized(*rows, out_dtype=dtype))
+        elif self.fused_norms:
+            f = self.ffn(norm.layer_norm(hidden_states, scale=c_scale, shift=c_shift, eps=self.norm3.eps))
+        else:
+            x = (self.norm3(hidden_states.float()) * (1 + c_scale) + c_shift).to(dtype)
+            f = self.ffn(x)
         return (hidden_states.float() + f.float() * c_gate).to(dtype)
 
 
@@ -176,6 +200,13 @@ class WanDiT(nn.Module):
         self.scale_shift_table = nn.Parameter(torch.randn(1, 2, dim) / dim ** 0.5)
         self.proj_out = nn.Linear(dim, cfg.out_channels * math.prod(cfg.patch_size))
         self._rope = None
+        self.fused_norms = False
+
+    def fuse_norms(self, on: bool = True) -> "WanDiT":
+        """Norms and modulations of every block and of the head as single passes on the GPU (off by default)."""
+        for m in (self, *self.blocks):
+            m.fused_norms = on
+        return self
 
     def rope(self, f: int, h: int, w: int, device):
         key = (f, h, w, str(device))
@@ -195,7 +226,10 @@ class WanDiT(nn.Module):
         for block in self.blocks:
             x = block(x, ctx, tproj, rotary, timestep=timestep)
         shift, scale = (self.scale_shift_table.float() + temb.float()[:, None]).chunk(2, dim=1)
-        x = (self.norm_out(x.float()) * (1 + scale) + shift).to(x.dtype)
+        if self.fused_norms:
+            x = norm.layer_norm(x, scale=scale, shift=shift, eps=self.norm_out.eps)
+        else:
+            x = (self.norm_out(x.float()) * (1 + scale) + shift).to(x.dtype)
         x = self.proj_out(x)
         x = x.reshape(b, f, h, w, pt, ph, pw, -1).permute(0, 7, 1, 4, 2, 5, 3, 6)
         return x.flatten(6, 7).flatten(4, 5).flatten(2, 3)

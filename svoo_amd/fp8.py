@@ -14,6 +14,7 @@ Values of a matrix ``[.., K]`` are stored as ``[.., 128 ceil(K / 128)]`` (zeros 
 * :func:`fp8_matmul`           ``a b^T + bias``, with the tanh GELU if asked for
 * :func:`fp8_linear`           ``x W^T + b`` from 16 or 32-bit tensors, differentiable
 * :class:`Fp8Linear`           a ``torch.nn.Linear``'s stand-in for inference, its weight laid out once
+* :class:`Fp8TrainLinear`      a ``torch.nn.Linear`` that computes by :func:`fp8_linear`
 
 NaN stays NaN and infinities become NaN in e4m3 (e5m2 keeps them); they do not count towards a block's scale.
 """
@@ -303,3 +304,21 @@ class Fp8Linear(torch.nn.Module):
     def extra_repr(self) -> str:
         return f"in_features={self.in_features}, out_features={self.out_features}, bias={self.bias is not None}, " \
                f"activation={self.activation}"
+
+
+class Fp8TrainLinear(torch.nn.Linear):
+    """A ``torch.nn.Linear`` that computes by :func:`fp8_linear`: parameters as the optimiser keeps them (bf16, fp16 or
+    fp32), quantised at every call."""
+
+    grad_dtype = torch.float8_e4m3fn
+
+    @classmethod
+    def from_linear(cls, linear: torch.nn.Linear, grad_dtype=torch.float8_e4m3fn) -> "Fp8TrainLinear":
+        """A layer that shares ``linear``'s parameters."""
+        _fp8_type(grad_dtype, "Fp8TrainLinear")
+        new = cls(linear.in_features, linear.out_features, bias=linear.bias is not None, device="meta")
+        new.weight, new.bias, new.grad_dtype = linear.weight, linear.bias, grad_dtype
+        return new.train(linear.training)
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        return fp8_linear(x, self.weight, self.bias, self.grad_dtype)

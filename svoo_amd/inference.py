@@ -12,12 +12,18 @@ No kernel warm-up is needed: the HIP kernels are compiled ahead of time.
 the same for HunyuanVideo 1.0 (``svoo/models/hunyuan10/inference.py:31-231``): one
 :class:`Hunyuan_SAPAttn_Processor` per double-stream block (layers ``0 .. D-1``), then per
 single-stream block (layers ``D ..``), the numbering the per-layer profile CSV is indexed by.
+
+``replace_wan_linear`` puts 8-bit linear layers into the blocks of a Wan pipeline; it has no counterpart in the reference.
 """
 
 from __future__ import annotations
 
 import os
 
+import torch
+
+from . import _lib
+from .fp8 import Fp8Linear, Fp8TrainLinear
 from .processor import (Hunyuan_SAPAttn_Processor, WanAttn_DenseAttn_Processor, WanAttn_EARAttn_Processor,
                         WanAttn_SAPAttn_Processor)
 from .sparsity import SparsityLookup
@@ -156,6 +162,72 @@ def replace_wan_attention(
                 block.attn1.set_processor(proc)
                 processors.append(proc)
     return processors
+
+
+def _plain_linear(m) -> bool:
+    """A ``torch.nn.Linear`` that nothing wraps or watches."""
+    return type(m) is torch.nn.Linear and not (m._forward_hooks or m._forward_pre_hooks or m._backward_hooks
+                                               or m._backward_pre_hooks or "forward" in m.__dict__)
+
+
+def _tanh_gelu(m) -> bool:
+    return type(m) is torch.nn.GELU and m.approximate == "tanh" and not (m._forward_hooks or m._forward_pre_hooks)
+
+
+def replace_wan_linear(pipe, trainable: bool = False, grad_dtype=torch.float8_e4m3fn):
+    """Put 8-bit linear layers into every block of a Wan pipeline's transformers (``transformer_2`` too).
+
+    Every plain ``torch.nn.Linear`` of a block's ``attn1``, ``attn2`` and ``ffn`` is replaced; embedders, modulation and
+    the head stay as they are, as do layers that something else wraps or hooks.  For inference
+    (:class:`svoo_amd.fp8.Fp8Linear`) the weight is laid out in 8 bits once and its original released, the query, key and
+    value projections of ``attn1`` become one ``to_qkv`` (``fused_projections``, which the processors here and in
+    diffusers know), and a tanh GELU behind the first ``ffn`` layer enters that layer's product.  With ``trainable``
+    (:class:`svoo_amd.fp8.Fp8TrainLinear`) layers share the parameters of those they replace and have gradients, the
+    incoming ones in ``grad_dtype``.  Weights have to be on the GPU.  Returns the new layers."""
+    transformers = [t for t in (pipe.transformer, getattr(pipe, "transformer_2", None)) if t is not None]
+    parts = [part for t in transformers for block in t.blocks
+             for part in (getattr(block, n, None) for n in ("attn1", "attn2", "ffn")) if part is not None]
+    for part in parts:  # before the first layer changes
+        for m in part.modules():
+            if _plain_linear(m):
+                _lib.elem_type(m.weight, "weight")
+    layers = []
+
+    def convert(linear, activation="none"):
+        new = Fp8TrainLinear.from_linear(linear, grad_dtype) if trainable else Fp8Linear.from_linear(linear, activation)
+        layers.append(new)
+        return new
+
+    def walk(parent):
+        kids = list(parent.named_children())
+        for i, (name, m) in enumerate(kids):
+            if _plain_linear(m):
+                fuse = not trainable and isinstance(parent, torch.nn.Sequential) and i + 1 < len(kids) and \
+                    _tanh_gelu(kids[i + 1][1])
+                setattr(parent, name, convert(m, "gelu_tanh" if fuse else "none"))
+                if fuse:
+                    setattr(parent, kids[i + 1][0], torch.nn.Identity())
+            elif type(m).__name__ == "GELU" and getattr(m, "approximate", None) == "tanh" and not trainable and \
+                    _plain_linear(getattr(m, "proj", None)):  # diffusers' projection with its GELU
+                setattr(parent, name, convert(m.proj, "gelu_tanh"))
+            else:
+                walk(m)
+
+    with torch.no_grad():
+        for t in transformers:
+            for block in t.blocks:
+                attn = getattr(block, "attn1", None)
+                qkv = [getattr(attn, n, None) for n in ("to_q", "to_k", "to_v")]
+                if not trainable and all(_plain_linear(m) for m in qkv) and not getattr(attn, "fused_projections", False) \
+                        and len({(m.in_features, m.weight.dtype, m.bias is None) for m in qkv}) == 1:
+                    bias = None if qkv[0].bias is None else torch.cat([m.bias for m in qkv])
+                    attn.to_qkv = Fp8Linear(torch.cat([m.weight for m in qkv]), bias)
+                    attn.fused_projections = True
+                    layers.append(attn.to_qkv)
+                    del attn.to_q, attn.to_k, attn.to_v
+        for part in parts:
+            walk(part)
+    return layers
 
 
 def _configure_profile(cls, use_dynamic_min_kc_ratio, sparsity_csv_path, dynamic_min_kc_ratio_min,

@@ -158,3 +158,30 @@ def test_fp8_refuses_in_python():
         fp8.fp8_linear(x, x)
     with pytest.raises(TypeError, match="float8"):
         fp8.fp8_linear(x, x, grad_dtype=torch.float16)
+    with pytest.raises(TypeError, match="float8"):
+        fp8.Fp8TrainLinear.from_linear(torch.nn.Linear(8, 8), grad_dtype=torch.bfloat16)
+
+
+@pytest.mark.parametrize("trainable", [False, True])
+def test_replace_wan_linear_leaves_a_pipeline_that_it_refuses(trainable):
+    from svoo_amd import dit
+    from svoo_amd.inference import replace_wan_linear
+
+    cfg = dit.WanDiTConfig(num_attention_heads=1, ffn_dim=64, num_layers=2, text_dim=32)
+    pipe = dit.make_pipe(cfg, dtype=torch.float32)
+    before = {n: id(m) for n, m in pipe.transformer.named_modules()}
+    with pytest.raises(AssertionError, match="GPU"):
+        replace_wan_linear(pipe, trainable=trainable)
+    assert {n: id(m) for n, m in pipe.transformer.named_modules()} == before
+    assert not pipe.transformer.fused_norms and not any(b.fused_norms for b in pipe.transformer.blocks)
+
+
+def test_train_linear_shares_parameters():
+    from svoo_amd import fp8
+
+    for bias in (True, False):
+        old = torch.nn.Linear(8, 16, bias=bias).eval()
+        new = fp8.Fp8TrainLinear.from_linear(old, torch.float8_e5m2)
+        assert new.weight is old.weight and new.bias is old.bias and new.grad_dtype == torch.float8_e5m2
+        assert (new.in_features, new.out_features, new.training) == (8, 16, False)
+        assert new.state_dict().keys() == old.state_dict().keys()
