@@ -127,12 +127,25 @@ __device__ __forceinline__ void buffer_dma16(i32x4_t buffer, uint32_t voff, uint
                    "s"(lds), "s"(soff), "i"(kAt)
                    : "memory", "scc");
 }
-// A byte per lane to words of LDS.
-template <int kAt>
-__device__ __forceinline__ void buffer_dma_bytes(i32x4_t buffer, uint32_t voff, uint32_t lds) {
-  __asm__ volatile("s_add_u32 m0, %2, %3\n\ts_nop 0\n\tbuffer_load_ubyte %0, %1, 0 offen lds" ::"v"(voff), "s"(buffer),
-                   "s"(lds), "i"(kAt)
-                   : "memory", "scc");
+// An element of 1, 2 or 4 bytes per lane to words of LDS.
+template <int kBytes, int kAt>
+__device__ __forceinline__ void buffer_dma_words(i32x4_t buffer, uint32_t voff, uint32_t lds) {
+  if constexpr (kBytes == 1)
+    __asm__ volatile("s_add_u32 m0, %2, %3\n\ts_nop 0\n\tbuffer_load_ubyte %0, %1, 0 offen lds" ::"v"(voff), "s"(buffer),
+                     "s"(lds), "i"(kAt)
+                     : "memory", "scc");
+  else if constexpr (kBytes == 2)
+    __asm__ volatile("s_add_u32 m0, %2, %3\n\ts_nop 0\n\tbuffer_load_ushort %0, %1, 0 offen lds" ::"v"(voff), "s"(buffer),
+                     "s"(lds), "i"(kAt)
+                     : "memory", "scc");
+  else
+    __asm__ volatile("s_add_u32 m0, %2, %3\n\ts_nop 0\n\tbuffer_load_dword %0, %1, 0 offen lds" ::"v"(voff), "s"(buffer),
+                     "s"(lds), "i"(kAt)
+                     : "memory", "scc");
+}
+template <class T>
+__device__ __forceinline__ const __attribute__((address_space(3))) T* lds_at(uint32_t at) {
+  return (const __attribute__((address_space(3))) T*)(uintptr_t)at;
 }
 // Until no more than N of the wave's loads and stores are outstanding, in a form that the compiler counts.
 template <int N>
@@ -259,6 +272,12 @@ __device__ __forceinline__ void store_rows32(const GemmArgs& g, f32x4_t (&acc)[F
 // The matrix instruction's first operand is b and its second a: a lane then holds four consecutive columns of a row of c.
 // The 16 x 16 x 128 form sustains 4.25 PFLOP/s from registers on random values, the 32 x 32 x 64 form 3.95: the clock
 // falls with the power that they take.
+//
+// What bounds it, kTile 256 (measured by stamps): per stage of 2048 matrix cycles 2500, 290 of them lost to barriers and to
+// instructions that wait for each other's issue, the rest to copies; per tile 9500 to add, pack and store 64K values, and
+// behind them the stores themselves (all blocks end a tile together), which at 1536 contracted positions take a third of
+// the time.  The clock is 1.8 GHz under random values and 2.3 under zeros.  8192^3 380 us (2.9 PFLOP/s),
+// 32760 x 1536 x 8960 335 us (2.7), 32760 x 8960 x 1536 430 us (2.1, 1.5 TB/s of stores), 8960 x 1536 x 32768 345 us (2.6).
 constexpr int kXcds = 8;
 constexpr int gemm_blocks(int tile) { return tile == 256 ? 256 : 512; }
 
@@ -298,7 +317,8 @@ fp8_gemm_tile_kernel(GemmArgs g) {
   constexpr int kCopies = kTile / 8 / kWaves;  // 1 KB copies per wave, stage and operand
   constexpr int kScaleBytes = 2 * kTile * 4, kScaleCopies = kTile / 128;  // a word per row of a and b and stage
   constexpr int kBand = 8;
-  __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * kStageBytes + 2 * kScaleBytes];
+  constexpr int kBiasAt = 2 * kStageBytes + 2 * kScaleBytes;
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[kBiasAt + kWaves * kPart * 4];
   const int lane = threadIdx.x % kWave, wave = uniform(threadIdx.x / kWave);
   const int wm = (wave / 2) * kPart, wn = (wave % 2) * kPart;
   const int mt = (g.m + kTile - 1) / kTile, nt = (g.n + kTile - 1) / kTile;
@@ -371,7 +391,7 @@ fp8_gemm_tile_kernel(GemmArgs g) {
   };
   auto copy_scales = [&](auto ic) __attribute__((always_inline)) {
     constexpr int i = decltype(ic)::value;
-    buffer_dma_bytes<i * kWaves * kWave * 4>(buf_s[i], vs[i] + s_k[i], s_dst);
+    buffer_dma_words<1, i * kWaves * kWave * 4>(buf_s[i], vs[i] + s_k[i], s_dst);
   };
   constexpr int kFirst = kCopies + kScaleCopies;
   auto copy_first = [&](auto ic) __attribute__((always_inline)) {
@@ -395,9 +415,8 @@ fp8_gemm_tile_kernel(GemmArgs g) {
   uint32_t s_at = lds_addr(lds) + 2 * kStageBytes + lane * 4, s_turn = kScaleBytes;
   auto read_scale = [&](auto ic) __attribute__((always_inline)) {
     constexpr int i = decltype(ic)::value;
-    typedef const __attribute__((address_space(3))) int* LdsInt;
-    if constexpr (i < kScales) na[i] = *(LdsInt)(s_at + (wm + i * kWave) * 4);
-    else nb[i - kScales] = *(LdsInt)(s_at + (kTile + wn + (i - kScales) * kWave) * 4);
+    if constexpr (i < kScales) na[i] = *lds_at<int>(s_at + (wm + i * kWave) * 4);
+    else nb[i - kScales] = *lds_at<int>(s_at + (kTile + wn + (i - kScales) * kWave) * 4);
   };
   auto word = [&](int v) __attribute__((always_inline)) {
     const auto x = __builtin_amdgcn_permlane16_swap(v, v, false, false);  // rows of 16 lanes 0 0 2 2, 1 1 3 3
@@ -411,25 +430,25 @@ fp8_gemm_tile_kernel(GemmArgs g) {
     else sb1[i - kScales] = word(nb[i - kScales]);
   };
 
-  // The bias: a lane loads that of a column or two of the wave's, an item ahead, in both widths without a branch.
-  constexpr int kBias = (kPart + kWave - 1) / kWave;
-  int raw[2 * kBias];
-  const __amdgpu_buffer_rsrc_t buf_bias = resource_from(
-      (const uint8_t*)g.bias, kShared || g.bias == nullptr ? 0 : (long long)g.n * (g.bias_type == kRowF32 ? 4 : 2));
-  auto load_bias = [&](const GemmPlace& p) __attribute__((always_inline)) {
-#pragma unroll
-    for (int i = 0; i < kBias; ++i) {
-      const int n = p.n0 + wn + i * kWave + lane;
-      raw[i] = __builtin_amdgcn_raw_buffer_load_b32(buf_bias, n * 4, 0, 0);
-      raw[kBias + i] = __builtin_amdgcn_raw_buffer_load_b16(buf_bias, n * 2, 0, 0);
-    }
+  // The bias of the wave's columns, copied at an item's start and read at its end, when it has landed long since (there are
+  // two stages at least).
+  const i32x4_t buf_bias =
+      buffer_from((const uint8_t*)g.bias, kShared || g.bias == nullptr ? 0 : (long long)g.n * (g.bias_type == kRowF32 ? 4 : 2));
+  const uint32_t bias_at = lds_addr(lds) + kBiasAt + wave * kPart * 4;
+  auto copy_bias = [&](int n0) __attribute__((always_inline)) {
+    if (g.bias_type == kRowF32) unroll<kScales>([&](auto ic) __attribute__((always_inline)) {
+      buffer_dma_words<4, decltype(ic)::value * kWave * 4>(buf_bias, (n0 + decltype(ic)::value * kWave + lane) * 4, bias_at);
+    });
+    else unroll<kScales>([&](auto ic) __attribute__((always_inline)) {
+      buffer_dma_words<2, decltype(ic)::value * kWave * 4>(buf_bias, (n0 + decltype(ic)::value * kWave + lane) * 2, bias_at);
+    });
   };
-  auto take_bias = [&](float (&bias)[kBias]) __attribute__((always_inline)) {
+  auto read_bias = [&](float (&bias)[kScales]) __attribute__((always_inline)) {
 #pragma unroll
-    for (int i = 0; i < kBias; ++i) {
-      const uint16_t half = (uint16_t)raw[kBias + i];
-      const float wide = g.bias_type == kRowBf16 ? bf16_to_f32(half) : (float)__builtin_bit_cast(_Float16, half);
-      bias[i] = g.bias_type == kRowF32 ? __int_as_float(raw[i]) : wide;
+    for (int i = 0; i < kScales; ++i) {
+      const int raw = *lds_at<int>(bias_at + (i * kWave + lane) * 4);
+      const float wide = g.bias_type == kRowBf16 ? bf16_to_f32((uint16_t)raw) : (float)__builtin_bit_cast(_Float16, (uint16_t)raw);
+      bias[i] = g.bias_type == kRowF32 ? __int_as_float(raw) : wide;
     }
   };
 
@@ -456,7 +475,7 @@ fp8_gemm_tile_kernel(GemmArgs g) {
   // Half e of operand r, or of one of the next stage's that waits for its registers.
   auto read = [&](auto rc, auto ec, i32x8_t& to) __attribute__((always_inline)) {
     constexpr int r = decltype(rc)::value, e = decltype(ec)::value;
-    const u32x4_t x = *(const __attribute__((address_space(3))) u32x4_t*)(off[r / F][r % 2][e] + r % F * 2048);
+    const u32x4_t x = *lds_at<u32x4_t>(off[r / F][r % 2][e] + r % F * 2048);
 #pragma unroll
     for (int i = 0; i < 4; ++i) to[4 * e + i] = (int)x[i];
   };
@@ -541,7 +560,8 @@ fp8_gemm_tile_kernel(GemmArgs g) {
       for (int k = 0; k < F; ++k) __asm__ volatile("" : "+a"(acc[i][k]));
   };
   // Until the copies of all but the last two half stages have landed, in all waves, and what those were read for before
-  // has left the stage's place.
+  // has left the stage's place.  (Behind a tile's end this waits for its stores too; counting them out gained nothing, as
+  // all blocks end their tiles together and the stores are bound by the memory.)
   auto turn = [&]() __attribute__((always_inline)) {
     wait_vmem<kFirst + kCopies>();
     __syncthreads();
@@ -550,7 +570,6 @@ fp8_gemm_tile_kernel(GemmArgs g) {
 
   GemmPlace p = place(walk.first);
   copy_from(source(p));
-  load_bias(p);
   unroll<kFirst>(copy_first);
   unroll<kCopies>(copy_second);
   copy_next();
@@ -571,6 +590,7 @@ fp8_gemm_tile_kernel(GemmArgs g) {
   for (int item = walk.first; item < walk.last; item += walk.step) {
     const GemmPlace next = place(item + walk.step < walk.last ? item + walk.step : item);
     const Source next_source = source(next);
+    if constexpr (!kShared) copy_bias(p.n0 + wn);
 #pragma unroll
     for (int i = 0; i < F; ++i)
 #pragma unroll
@@ -594,9 +614,8 @@ fp8_gemm_tile_kernel(GemmArgs g) {
       copy_next();
     }
     hold_sums();
-    float bias[kBias];
-    take_bias(bias);
-    load_bias(next);
+    float bias[kScales];
+    if constexpr (!kShared) read_bias(bias);
     const int m0 = p.m0 + wm, n0 = p.n0 + wn;
     if constexpr (kShared || C == kRowF32) {
       store_rows32<kShared>(g, acc, m0, n0, p.split, bias);

@@ -109,17 +109,22 @@ struct GemmPlan {
 
 // The kernel and the number of shares with the shortest estimated time, in microseconds: rounds of items over the blocks
 // that run at a time, each its stages and a constant for its start and end; shares add the partial sums' way out and back.
+// Two blocks of 128 x 128 share a CU, and a round of no more than 256 has the CUs to itself.  Fitted to both tiles at 24
+// sizes, e.g. (256 against 128) 2048 x 5120 x 5120 58 and 62 us, 4096 x 5120 x 5120 117 and 102, 32760 x 1536 x 8960 341 and
+// 437, 2048 x 1536 x 8960 82 and 38; what it picks there is within a tenth of the faster.
 static GemmPlan gemm_plan(long long m, long long n, long long kb, bool wide) {
   if (m <= 64) return {0, 1};
   GemmPlan best = {128, 1};
   double best_us = 1e30;
   for (int tile = wide ? 128 : 256; tile >= 128; tile -= 128) {
-    const long long tiles = ((m + tile - 1) / tile) * ((n + tile - 1) / tile);
-    const double stage = tile == 256 ? 1.1 : wide ? 1.4 : 0.75, ends = tile == 256 ? 8.0 : 4.0;
+    const long long tiles = ((m + tile - 1) / tile) * ((n + tile - 1) / tile), blocks = gemm_blocks(tile);
+    const double stage = tile == 256 ? 1.25 : wide ? 1.4 : 0.95, alone = tile == 256 || wide ? stage : 0.5;
+    const double ends = tile == 256 ? 8.0 : 4.0;
     for (int splits = 1; splits <= 32 && (splits == 1 || kb / splits >= 2); ++splits) {
-      const long long rounds = (tiles * splits + gemm_blocks(tile) - 1) / gemm_blocks(tile);
-      double us = rounds * ((double)((kb + splits - 1) / splits) * stage + ends);
-      if (splits > 1) us += 4.0 + (double)m * n * splits * 8.0 / 4e6;
+      const long long items = tiles * splits, left = items % blocks, stages = (kb + splits - 1) / splits;
+      double us = (items / blocks) * (stages * stage + ends);
+      if (left > 0) us += stages * (left <= 256 ? alone : stage) + ends;
+      if (splits > 1) us += 5.0 + (double)m * n * splits * 8.0 / 6e6;
       if (us < best_us) {
         best_us = us;
         best = {tile, splits};
