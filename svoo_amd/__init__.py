@@ -16,6 +16,17 @@ from .co_clustering import (  # noqa: F401
     triton_l2norm_forward,
     weighted_softmax,
 )
+from .fp8 import (  # noqa: F401
+    Fp8Linear,
+    Fp8TrainLinear,
+    fp8_dequantize,
+    fp8_linear,
+    fp8_matmul,
+    fp8_quantize_blocks,
+    fp8_quantize_both,
+    fp8_quantize_rows,
+)
+from .norm import layer_norm, layer_norm_bwd, layer_norm_fp8, layer_norm_fwd  # noqa: F401
 from .permute import (  # noqa: F401
     apply_inverse_permutation,
     apply_inverse_permutation_triton,

@@ -8,7 +8,7 @@ namespace svoo {
 // with 46 of them at 1536 columns eight waves a SIMD keep enough loads in flight.  A block's rows share a batch entry,
 // whose parameters lie in LDS: in registers they would take more than the row, and loaded per row twice its bytes.
 // Measured, modulated bf16: 32760 x 1536 36 us (5.6 TB/s; 66 us with parameters and the row's values in fp32 registers),
-// 75600 x 5120 310 us (5.0 TB/s; 777 us).  Over widths of 128 to 8192 in whole chunks 4.0 to 5.2 TB/s, a wave per row
+// 75600 x 5120 310 us (5.0 TB/s; 777 us).  Over other widths in whole chunks 3.7 to 5.2 TB/s (3.1 to 3.4 at 64 and 256), a wave per row
 // 20% above a block of 256 per row at 5120; rows of an odd length above 1536 columns, element by element at the end and
 // with no chunk on a 16-byte address, 1.8 to 3.3 TB/s.
 template <int T, int TPR, int NC, bool kWhole, bool kFp8>

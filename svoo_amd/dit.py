@@ -108,11 +108,16 @@ class WanAttention(nn.Module):
         return self.processor(self, hidden_states, encoder_hidden_states, attention_mask, rotary_emb, timestep)
 
 
+def _watched(*modules) -> bool:
+    """Hooks wait for a call of one of the modules."""
+    return any(m._forward_hooks or m._forward_pre_hooks or m._backward_hooks or m._backward_pre_hooks for m in modules)
+
+
 class WanBlock(nn.Module):
     """One Wan DiT block: modulated self-attention, cross-attention to the text, modulated FFN.
 
-    With ``fused_norms`` each norm and its modulation are one pass (:func:`svoo_amd.norm.layer_norm`, differentiable),
-    and an 8-bit FFN (:func:`svoo_amd.inference.replace_wan_linear`) takes its input as 8-bit rows from the norm."""
+    With ``fused_norms`` each norm and its modulation are one pass (:func:`svoo_amd.norm.layer_norm`, differentiable) in
+    place of the norm modules' calls, and an 8-bit FFN (:func:`svoo_amd.inference.replace_wan_linear`) takes its input as 8-bit rows from the norm."""
 
     fused_norms = False
 
@@ -143,9 +148,12 @@ class WanBlock(nn.Module):
         else:
             x = self.norm2(hidden_states.float()).to(dtype)
         hidden_states = hidden_states + self.attn2(hidden_states=x, encoder_hidden_states=encoder_hidden_states)
-        if self.fused_norms and isinstance(self.ffn[0], Fp8Linear):
+        if self.fused_norms and isinstance(self.ffn[0], Fp8Linear) and not _watched(self.ffn, self.ffn[0]):
             rows = norm.layer_norm_fp8(hidden_states, scale=c_scale, shift=c_shift, eps=self.norm3.eps)
-            f = self.ffn[1:](self.ffn[0].forward_quantized(*rows, out_dtype=dtype))
+            first, *rest = self.ffn
+            f = first.forward_quantized(*rows, out_dtype=dtype)
+            for layer in rest:
+                f = layer(f)
         elif self.fused_norms:
             f = self.ffn(norm.layer_norm(hidden_states, scale=c_scale, shift=c_shift, eps=self.norm3.eps))
         else:

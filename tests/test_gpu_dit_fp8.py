@@ -267,7 +267,28 @@ def test_what_is_replaced(gpu):
     assert type(b[1]) is Wrapped and c[1] is hooked
     assert isinstance(c[0][0], fp8.Fp8Linear) and c[0][0].activation == "none" and type(c[0][1]) is nn.GELU
     assert layers == [a[0], a[1], b[0].proj, c[0][0]]
+    assert replace_wan_linear(SimpleNamespace(transformer=SimpleNamespace(blocks=blocks))) == []  # nothing is left to do
     with torch.no_grad():
         want = fp8.fp8_matmul(*fp8.fp8_quantize_rows(x), *fp8.fp8_quantize_blocks(first.weight), bias=first.bias,
                               activation="gelu_tanh")
         assert torch.equal(a[0](x), want)
+
+
+def test_hooks_on_the_ffn_are_called(gpu):
+    """A hook on the FFN or on its first layer gets its call; the values are those of the layers one after the other."""
+    from svoo_amd.inference import replace_wan_linear
+
+    pipe = _pipe(gpu, 1, 1)
+    replace_wan_linear(pipe)
+    block = pipe.transformer.fuse_norms().blocks[0]
+    for a in (block.attn1, block.attn2):
+        a.set_processor(Mix())
+    x, ctx, temb = _inputs(pipe.transformer.config, gpu, 1, 50)
+    with torch.no_grad():
+        want = block(x, ctx, temb, None)
+        for module in (block.ffn, block.ffn[0]):
+            seen = []
+            handle = module.register_forward_hook(lambda m, args, out: seen.append(args[0].dtype))
+            assert torch.equal(block(x, ctx, temb, None), want)  # quantised in the norm or behind it: the same values
+            handle.remove()
+            assert seen == [BF16]

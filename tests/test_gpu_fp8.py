@@ -143,6 +143,20 @@ def test_product_of_whole_numbers_is_exact(gpu, m, n, k):
         assert c.shape == (m, n) and torch.equal(c, want.to(out))
 
 
+@pytest.mark.parametrize("m,n,k", [(3, 77, 256), (300, 129, 200), (513, 1025, 640), (512, 1536, 4096), (9000, 9007, 128),
+                                   (5120, 5000, 1100), (7777, 5121, 640), (1500, 1290, 20100)])
+def test_product_with_a_bias_is_exact(gpu, m, n, k):
+    """The bias, a whole number below 8, adds to the sums above without a rounding either: every column gets its own."""
+    from svoo_amd import fp8
+
+    for i, (bias_type, out) in enumerate([(BF16, BF16), (F16, F32), (F32, F16), (F32, F32)]):
+        qa, sa, qb, sb, va, vb = _whole(m + n + k + i, gpu, m, n, k, (1, 128)[i % 2], E4)
+        bias = torch.randint(-8, 9, (n,), device=gpu, generator=torch.Generator(device=gpu).manual_seed(i)).to(bias_type)
+        say("whole, bias", m, n, k, bias_type, out)
+        c = fp8.fp8_matmul(qa, sa, qb, sb, bias, out_dtype=out)
+        assert torch.equal(c, (va @ vb.t() + bias.double()).to(out))
+
+
 @pytest.mark.parametrize("m,n,k", [(1, 700, 1000), (40, 300, 520), (300, 500, 1000), (1000, 2000, 3000)])
 @pytest.mark.parametrize("out", [BF16, F16, F32])
 def test_product_of_random_matrices(gpu, m, n, k, out):

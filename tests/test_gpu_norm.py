@@ -295,3 +295,18 @@ def test_norm_on_other_streams_and_in_a_graph(gpu):
         torch.cuda.synchronize()
         assert all(torch.equal(u, v) for u, v in zip(out, ref)), i
         assert all(torch.equal(u, v) for u, v in zip(step(x2, dy2), want2))
+
+
+@pytest.mark.parametrize("cols", [40, 128, 500, 999, 1536, 1543, 2048, 4096, 5000, 8200, 16384])
+def test_norm_gradients_of_other_types(gpu, cols):
+    """An incoming gradient of another type than x's: y was asked for in that type."""
+    from svoo_amd import norm
+
+    for seed, (dtype, dy_dtype) in enumerate([(BF16, F32), (BF16, F16), (F16, BF16), (F16, F32), (F32, BF16), (F32, F16)]):
+        x, dy, p = _inputs(seed, gpu, 2, 21, cols, dtype, "modulated" if seed % 2 else "affine", F32)
+        dy = dy.to(dy_dtype)
+        say("norm, dy of another type", cols, dtype, dy_dtype)
+        y, mean, rstd = norm.layer_norm_fwd(x, out_dtype=dy_dtype, **p)
+        assert y.dtype == dy_dtype
+        _check_forward(y, x, p, 1e-6)
+        _check_backward(norm.layer_norm_bwd(dy, x, mean, rstd, **p), x, dy, p, 1e-6)
