@@ -94,19 +94,6 @@ __device__ __forceinline__ u32x4_t pack_rows(f32x4_t left, f32x4_t right) {
   return v;
 }
 
-// The first n (or all) of eight 16-bit elements to any address.
-__device__ __forceinline__ void store_row8_bits(uint16_t* p, int n, u32x4_t v) {
-  if (n >= 8) {
-    ((Dwords4*)p)->v = v;
-  } else if (n > 0) {
-    if (n & 4) *(Dwords2*)p = Dwords2{{v[0], v[1]}};
-    const uint32_t two = n & 4 ? v[2] : v[0], one = n & 2 ? (n & 4 ? v[3] : v[1]) : two;
-    p += n & 4;
-    if (n & 2) *(Dword*)p = Dword{two};
-    if (n & 1) p[n & 2] = (uint16_t)one;
-  }
-}
-
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
 // A matrix from one of its rows on, as a buffer resource: reads past its end give zeros.

@@ -9,8 +9,9 @@ namespace svoo {
 // whose parameters lie in LDS: in registers they would take more than the row, and loaded per row twice its bytes.
 // Measured, modulated bf16: 32760 x 1536 36 us (5.6 TB/s; 66 us with parameters and the row's values in fp32 registers),
 // 75600 x 5120 310 us (5.0 TB/s; 777 us).  Over other widths in whole chunks 3.7 to 5.2 TB/s (3.1 to 3.4 at 64 and 256), a wave per row
-// 20% above a block of 256 per row at 5120; rows of an odd length above 1536 columns, element by element at the end and
-// with no chunk on a 16-byte address, 1.8 to 3.3 TB/s.
+// 20% above a block of 256 per row at 5120; bf16 rows of an odd length, with no
+// chunk on a 16-byte address, 2.8 to 4.5 TB/s (to 8 bits 1.2 to 3.3); the last chunk is loaded as the row's last eight and
+// moved down, 2561 columns 284 us where element by element and a block per row took 587.
 template <int T, int TPR, int NC, bool kWhole, bool kFp8>
 __device__ __forceinline__ void norm_rows(const NormArgs& a, const f32x4_t* w, const f32x4_t* b, float2* scratch) {
   const int groups = blockDim.x / TPR, t = threadIdx.x % TPR;
@@ -18,9 +19,11 @@ __device__ __forceinline__ void norm_rows(const NormArgs& a, const f32x4_t* w, c
   const float inv = 1.0f / (float)a.cols;
   int half = 0;
   for (unsigned r = part * groups + threadIdx.x / TPR; r < a.rows_per_batch; r += a.parts * groups) {
+    int cols = a.cols;
+    if (!kWhole) __asm__ volatile("" : "+s"(cols));  // masks of the row's end made here: held over the rows they spill
     const size_t row = (size_t)batch * a.rows_per_batch + r;
     RawRow<T, NC> x;
-    x.template load<TPR, kWhole>(a.x, batch * a.x_batch + r * a.x_row, a.cols, t);
+    x.template load<TPR, kWhole>(a.x, batch * a.x_batch + r * a.x_row, cols, t);
     float s0 = 0.0f, s1 = 0.0f;
 #pragma unroll
     for (int c = 0; c < NC; ++c)
@@ -42,11 +45,11 @@ __device__ __forceinline__ void norm_rows(const NormArgs& a, const f32x4_t* w, c
       float u1 = 0.0f, u2 = 0.0f;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const float d = kWhole || col + e < a.cols ? x.at(c, e) - mean0 : 0.0f;
+        const float d = kWhole || col + e < cols ? x.at(c, e) - mean0 : 0.0f;
         u1 += d;
         u2 = fmaf(d, d, u2);
       }
-      const bool in = !kWhole || col < a.cols;
+      const bool in = !kWhole || col < cols;
       d1 += in ? u1 : 0.0f;
       d2 += in ? u2 : 0.0f;
     }
@@ -58,7 +61,7 @@ __device__ __forceinline__ void norm_rows(const NormArgs& a, const f32x4_t* w, c
       if (a.rstd != nullptr) a.rstd[row] = rstd;
     }
     x.forget();
-    const int blocks = (a.cols + 127) / 128;
+    const int blocks = (cols + 127) / 128;
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
       const int col = (c * TPR + t) * 8;
@@ -70,13 +73,13 @@ __device__ __forceinline__ void norm_rows(const NormArgs& a, const f32x4_t* w, c
         for (int e = 0; e < 4; ++e) y[4 * h + e] = fmaf((x.at(c, 4 * h + e) - mean0 - dm) * rstd, wv[e], bv[e]);
       }
       if (!kFp8) {
-        store_row8_as<kWhole>(a.y, a.y_type, (long long)row * a.cols + col, a.cols - col, y);
+        store_row8_as<kWhole>(a.y, a.y_type, (long long)row * cols + col, cols - col, y);
       } else {
         // the rounded row, as a quantiser of the stored one would see it; 16 lanes hold a block of 128 columns
         float amax = 0.0f;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          y[e] = col + (kWhole ? 0 : e) < a.cols ? row_round(a.y_type, y[e]) : 0.0f;
+          y[e] = col + (kWhole ? 0 : e) < cols ? row_round(a.y_type, y[e]) : 0.0f;
           amax = fmaxf(amax, finite_abs(y[e]));
         }
         const int e8 = block_exponent(max16(amax), a.fp8);
@@ -136,7 +139,7 @@ static void for_width(int cols, F f) {
   else if (whole && cols <= 1024) f(std::integral_constant<int, 64>(), std::integral_constant<int, 2>());
   else if (cols <= 1536) f(std::integral_constant<int, 64>(), std::integral_constant<int, 3>());
   else if (whole && cols <= 2560) f(std::integral_constant<int, 64>(), std::integral_constant<int, 5>());
-  else if (whole && cols <= 5120) f(std::integral_constant<int, 64>(), std::integral_constant<int, 10>());
+  else if (cols <= 5120) f(std::integral_constant<int, 64>(), std::integral_constant<int, 10>());
   else if (cols <= 8192) f(std::integral_constant<int, 1024>(), std::integral_constant<int, 1>());
   else f(std::integral_constant<int, 1024>(), std::integral_constant<int, 2>());
 }
@@ -200,7 +203,7 @@ extern "C" int svoo_layer_norm_fwd(const void* x, int x_type, long long x_batch_
     for_type(x_type, [&](auto type) {
       for_flag(cols % 8 == 0, [&](auto whole) {
         constexpr bool kWhole = decltype(whole)::value;
-        if constexpr (kWhole || kNc == 1 || kNc == 3 || kTpr == 1024) {
+        if constexpr (kWhole || kNc == 1 || kNc == 3 || kNc == 10 || kTpr == 1024) {
           for_flag(q != nullptr, [&](auto to_fp8) {
             hipLaunchKernelGGL((norm_fwd_kernel<decltype(type)::value, kTpr, kNc, kWhole, decltype(to_fp8)::value>), grid,
                                block, 0, (hipStream_t)stream, a);

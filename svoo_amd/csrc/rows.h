@@ -58,31 +58,48 @@ __device__ __forceinline__ void load_row8(const void* p, long long i, int n, flo
   }
 }
 
+// The first n (or all) of eight 16-bit elements to any address.
+__device__ __forceinline__ void store_row8_bits(uint16_t* p, int n, u32x4_t v) {
+  if (n >= 8) {
+    ((Dwords4*)p)->v = v;
+  } else if (n > 0) {
+    if (n & 4) *(Dwords2*)p = Dwords2{{v[0], v[1]}};
+    const uint32_t two = n & 4 ? v[2] : v[0], one = n & 2 ? (n & 4 ? v[3] : v[1]) : two;
+    p += n & 4;
+    if (n & 2) *(Dword*)p = Dword{two};
+    if (n & 1) p[n & 2] = (uint16_t)one;
+  }
+}
+
 template <int T, bool kWhole = false>
 __device__ __forceinline__ void store_row8(void* p, long long i, int n, const float (&f)[8]) {
-  if (n >= 8) {
-    if (T == kRowF32) {
-      ((Dwords4*)((float*)p + i))->v = u32x4_t{__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]),
-                                               __float_as_uint(f[3])};
-      ((Dwords4*)((float*)p + i + 4))->v = u32x4_t{__float_as_uint(f[4]), __float_as_uint(f[5]), __float_as_uint(f[6]),
-                                                   __float_as_uint(f[7])};
-    } else {
-      u32x4_t w;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        if (T == kRowBf16) {
-          w[e] = cvt_pk_bf16(f[2 * e], f[2 * e + 1]);
-        } else {
-          w[e] = (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)f[2 * e]) |
-                 ((uint32_t)__builtin_bit_cast(uint16_t, (_Float16)f[2 * e + 1]) << 16);
-        }
-      }
-      ((Dwords4*)((uint16_t*)p + i))->v = w;
+  if (T == kRowF32) {
+    float* to = (float*)p + i;
+    const u32x4_t a = {__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3])};
+    const u32x4_t b = {__float_as_uint(f[4]), __float_as_uint(f[5]), __float_as_uint(f[6]), __float_as_uint(f[7])};
+    if (n >= 8) {
+      ((Dwords4*)to)->v = a;
+      ((Dwords4*)(to + 4))->v = b;
+    } else if (!kWhole && n > 0) {
+      if (n & 4) ((Dwords4*)to)->v = a;
+      const u32x4_t rest = n & 4 ? b : a;
+      to += n & 4;
+      if (n & 2) *(Dwords2*)to = Dwords2{{rest[0], rest[1]}};
+      if (n & 1) *(Dword*)(to + (n & 2)) = Dword{n & 2 ? rest[2] : rest[0]};
     }
-  } else if (!kWhole) {
+  } else {
+    u32x4_t w;
 #pragma unroll
-    for (int e = 0; e < 8; ++e)
-      if (e < n) set_row_elem(p, T, i + e, f[e]);
+    for (int e = 0; e < 4; ++e) {
+      if (T == kRowBf16) {
+        w[e] = cvt_pk_bf16(f[2 * e], f[2 * e + 1]);
+      } else {
+        w[e] = (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)f[2 * e]) |
+               ((uint32_t)__builtin_bit_cast(uint16_t, (_Float16)f[2 * e + 1]) << 16);
+      }
+    }
+    if (n >= 8) ((Dwords4*)((uint16_t*)p + i))->v = w;
+    else if (!kWhole) store_row8_bits((uint16_t*)p + i, n, w);
   }
 }
 
@@ -108,7 +125,9 @@ struct RawRow {
       } else {
 #pragma unroll
         for (int h = 0; h < (T == kRowF32 ? 2 : 1); ++h) v[c][h] = u32x4_t{0, 0, 0, 0};
-        if (!kWhole) {
+        if (!kWhole && TPR > 16) {  // more than eight columns: the last eight, moved down
+          if (n > 0) load_end(v[c], p, i + n - 8, 8 - n);
+        } else if (!kWhole) {
 #pragma unroll
           for (int e = 0; e < 8; ++e)
             if (e < n) {
@@ -117,6 +136,30 @@ struct RawRow {
             }
         }
       }
+    }
+  }
+  // Elements i + by .. i + 7 to the front, zeros behind; by is 1 to 7.
+  static __device__ __forceinline__ void load_end(u32x4_t (&to)[T == kRowF32 ? 2 : 1], const void* p, long long i, int by) {
+    if (T == kRowF32) {
+      const u32x4_t a = ((const Dwords4*)((const float*)p + i))->v, b = ((const Dwords4*)((const float*)p + i + 4))->v;
+      uint32_t w[8] = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+#pragma unroll
+      for (int step = 4; step > 0; step /= 2)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) w[e] = by & step ? (e + step < 8 ? w[e + step < 8 ? e + step : 0] : 0u) : w[e];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) to[T == kRowF32 ? e / 4 : 0][e % 4] = w[e];
+    } else {
+      const u32x4_t a = ((const Dwords4*)((const uint16_t*)p + i))->v;
+      unsigned long long lo = a[0] | (unsigned long long)a[1] << 32, hi = a[2] | (unsigned long long)a[3] << 32;
+      if (by >= 4) {
+        lo = hi;
+        hi = 0;
+      }
+      const int bits = by % 4 * 16;
+      lo = lo >> bits | (bits ? hi << (64 - bits) : 0ull);
+      hi >>= bits;
+      to[0] = u32x4_t{(uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32)};
     }
   }
   // Values converted before are converted again: held in fp32 they would take the registers that this type saves.
