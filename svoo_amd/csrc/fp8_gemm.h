@@ -264,7 +264,7 @@ __device__ __forceinline__ void store_rows32(const GemmArgs& g, f32x4_t (&acc)[F
 // instructions that wait for each other's issue, the rest to copies; per tile 9500 to add, pack and store 64K values, and
 // behind them the stores themselves (all blocks end a tile together), which at 1536 contracted positions take a third of
 // the time.  The clock is 1.8 GHz under random values and 2.3 under zeros.  8192^3 380 us (2.9 PFLOP/s),
-// 32760 x 1536 x 8960 335 us (2.7), 32760 x 8960 x 1536 430 us (2.1, 1.5 TB/s of stores), 8960 x 1536 x 32768 345 us (2.6).
+// 32760 x 1536 x 8960 330 us (2.7), 32760 x 8960 x 1536 415 us (2.2, 1.4 TB/s of stores), 8960 x 1536 x 32768 350 us (2.6).
 constexpr int kXcds = 8;
 constexpr int gemm_blocks(int tile) { return tile == 256 ? 256 : 512; }
 
@@ -303,7 +303,8 @@ fp8_gemm_tile_kernel(GemmArgs g) {
   constexpr int kStageBytes = 2 * kTile * 128;
   constexpr int kCopies = kTile / 8 / kWaves;  // 1 KB copies per wave, stage and operand
   constexpr int kScaleBytes = 2 * kTile * 4, kScaleCopies = kTile / 128;  // a word per row of a and b and stage
-  constexpr int kBand = 8;
+  // 4, 5, 6, 8, 11 and 16 rows of 256: 391, 397, 400, 406, 415 and 420 us at 32760 x 1536 x 8960, within 2% elsewhere
+  constexpr int kBand = kTile == 256 ? 4 : 8;
   constexpr int kBiasAt = 2 * kStageBytes + 2 * kScaleBytes;
   __shared__ __attribute__((aligned(1024))) uint8_t lds[kBiasAt + kWaves * kPart * 4];
   const int lane = threadIdx.x % kWave, wave = uniform(threadIdx.x / kWave);
