@@ -117,7 +117,8 @@ class WanBlock(nn.Module):
     """One Wan DiT block: modulated self-attention, cross-attention to the text, modulated FFN.
 
     With ``fused_norms`` each norm and its modulation are one pass (:func:`svoo_amd.norm.layer_norm`, differentiable) in
-    place of the norm modules' calls, and an 8-bit FFN (:func:`svoo_amd.inference.replace_wan_linear`) takes its input as 8-bit rows from the norm."""
+    place of the norm modules' calls, and an 8-bit FFN (:func:`svoo_amd.inference.replace_wan_linear`) takes its input as
+    8-bit rows from the norm."""
 
     fused_norms = False
 

@@ -164,14 +164,19 @@ def replace_wan_attention(
     return processors
 
 
+def _unwatched(m) -> bool:
+    """No hook waits for a call of the module, and its ``forward`` is its class's."""
+    return not (m._forward_hooks or m._forward_pre_hooks or m._backward_hooks or m._backward_pre_hooks
+                or "forward" in m.__dict__)
+
+
 def _plain_linear(m) -> bool:
     """A ``torch.nn.Linear`` that nothing wraps or watches."""
-    return type(m) is torch.nn.Linear and not (m._forward_hooks or m._forward_pre_hooks or m._backward_hooks
-                                               or m._backward_pre_hooks or "forward" in m.__dict__)
+    return type(m) is torch.nn.Linear and _unwatched(m)
 
 
 def _tanh_gelu(m) -> bool:
-    return type(m) is torch.nn.GELU and m.approximate == "tanh" and not (m._forward_hooks or m._forward_pre_hooks)
+    return type(m) is torch.nn.GELU and m.approximate == "tanh" and _unwatched(m)
 
 
 def replace_wan_linear(pipe, trainable: bool = False, grad_dtype=torch.float8_e4m3fn):
@@ -208,7 +213,7 @@ def replace_wan_linear(pipe, trainable: bool = False, grad_dtype=torch.float8_e4
                 if fuse:
                     setattr(parent, kids[i + 1][0], torch.nn.Identity())
             elif type(m).__name__ == "GELU" and getattr(m, "approximate", None) == "tanh" and not trainable and \
-                    _plain_linear(getattr(m, "proj", None)):  # diffusers' projection with its GELU
+                    _unwatched(m) and _plain_linear(getattr(m, "proj", None)):  # diffusers' projection with its GELU
                 setattr(parent, name, convert(m.proj, "gelu_tanh"))
             else:
                 walk(m)

@@ -256,7 +256,9 @@ def test_what_is_replaced(gpu):
     blocks = nn.ModuleList([Block([GELU("tanh"), nn.Linear(256, 128)]), Block([GELU("none"), Wrapped(256, 128)])])
     hooked = nn.Linear(256, 128)
     hooked.register_forward_hook(lambda *a: None)
-    blocks.append(Block([nn.Sequential(nn.Linear(128, 256), nn.GELU()), hooked]))
+    watched = GELU("tanh")  # its own call is waited for: only the layer inside may change
+    watched.register_forward_pre_hook(lambda *a: None)
+    blocks.append(Block([nn.Sequential(nn.Linear(128, 256), nn.GELU()), hooked, watched]))
     blocks.to(gpu, BF16)
     x = torch.randn(5, 128, generator=torch.Generator(device=gpu).manual_seed(2), device=gpu).to(BF16)
     first = blocks[0].ffn[0].proj
@@ -266,7 +268,8 @@ def test_what_is_replaced(gpu):
     assert type(b[0]) is GELU and isinstance(b[0].proj, fp8.Fp8Linear) and b[0].proj.activation == "none"
     assert type(b[1]) is Wrapped and c[1] is hooked
     assert isinstance(c[0][0], fp8.Fp8Linear) and c[0][0].activation == "none" and type(c[0][1]) is nn.GELU
-    assert layers == [a[0], a[1], b[0].proj, c[0][0]]
+    assert c[2] is watched and watched.proj.activation == "none"
+    assert layers == [a[0], a[1], b[0].proj, c[0][0], watched.proj]
     assert replace_wan_linear(SimpleNamespace(transformer=SimpleNamespace(blocks=blocks))) == []  # nothing is left to do
     with torch.no_grad():
         want = fp8.fp8_matmul(*fp8.fp8_quantize_rows(x), *fp8.fp8_quantize_blocks(first.weight), bias=first.bias,
