@@ -283,7 +283,7 @@ int svoo_exact_sparsity_counts(const uint16_t* scores, long long rows, int n, fl
  *   y = n w + b, or with `modulated` y = n (1 + w) + b.  w and b ([cols] per batch entry, 0 as the batch stride for shared
  *   ones, NULL for none) and every other tensor have an element type: 0 bf16, 1 fp16, 2 fp32.
  *   svoo_layer_norm_fwd: y [batch * rows_per_batch][cols], or instead 8-bit rows q and q_scale as svoo_fp8_quantize_rows
- *     makes them (fp8_type) of the y that y_type would hold; mean and rstd (fp32, one per row) are optional.
+ *     makes them (fp8_type) of the y that y_type, here x's type, would hold; mean and rstd (fp32, one per row) are optional.
  *   svoo_layer_norm_bwd: dx (type of x, contiguous), dw and db ([batch][cols]; pass batch 1 for shared parameters), each
  *     optional.  The sums over rows are fp32 in a fixed order.
  * Beside the norms and modulation of svoo/models/wan/custom_models.py:23-109.

@@ -8,10 +8,10 @@ namespace svoo {
 // with 46 of them at 1536 columns eight waves a SIMD keep enough loads in flight.  A block's rows share a batch entry,
 // whose parameters lie in LDS: in registers they would take more than the row, and loaded per row twice its bytes.
 // Measured, modulated bf16: 32760 x 1536 36 us (5.6 TB/s; 66 us with parameters and the row's values in fp32 registers),
-// 75600 x 5120 310 us (5.0 TB/s; 777 us).  Over other widths in whole chunks 3.7 to 5.2 TB/s (3.1 to 3.4 at 64 and 256), a wave per row
-// 20% above a block of 256 per row at 5120; bf16 rows of an odd length, with no
-// chunk on a 16-byte address, 2.8 to 4.5 TB/s (to 8 bits 1.2 to 3.3); the last chunk is loaded as the row's last eight and
-// moved down, 2561 columns 284 us where element by element and a block per row took 587.
+// 75600 x 5120 310 us (5.0 TB/s; 777 us); to 8 bits 32760 x 1536 43 us (3.5 TB/s), bound by its arithmetic as well.
+// Over other widths in whole chunks 3.7 to 5.2 TB/s (3.1 to 3.4 at 64 and 256); bf16 rows of an odd length, with no chunk
+// on a 16-byte address, 2.8 to 4.5 TB/s (to 8 bits 1.8 to 3.9): the last chunk is loaded as the row's last eight and moved
+// down (104816 x 2561 270 us; element by element, with a block per row, 587).
 template <int T, int TPR, int NC, bool kWhole, bool kFp8>
 __device__ __forceinline__ void norm_rows(const NormArgs& a, const f32x4_t* w, const f32x4_t* b, float2* scratch) {
   const int groups = blockDim.x / TPR, t = threadIdx.x % TPR;
@@ -66,23 +66,36 @@ __device__ __forceinline__ void norm_rows(const NormArgs& a, const f32x4_t* w, c
     for (int c = 0; c < NC; ++c) {
       const int col = (c * TPR + t) * 8;
       float y[8];
+      bool in = true;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const f32x4_t wv = w[(c * 2 + h) * TPR + t], bv = b[(c * 2 + h) * TPR + t];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) y[4 * h + e] = fmaf((x.at(c, 4 * h + e) - mean0 - dm) * rstd, wv[e], bv[e]);
+        for (int e = 0; e < 4; ++e) {
+          y[4 * h + e] = fmaf((x.at(c, 4 * h + e) - mean0 - dm) * rstd, wv[e], bv[e]);
+          __asm__("" : "+v"(y[4 * h + e]));  // an fp32 number in every kernel: some would round to fp16 in the same step
+        }
       }
       if (!kFp8) {
         store_row8_as<kWhole>(a.y, a.y_type, (long long)row * cols + col, cols - col, y);
       } else {
-        // the rounded row, as a quantiser of the stored one would see it; 16 lanes hold a block of 128 columns
+        // the row rounded to x's type, as a quantiser of the stored one would see it; 16 lanes hold a block of 128 columns
+        round_row8<T>(y);
         float amax = 0.0f;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          y[e] = col + (kWhole ? 0 : e) < cols ? row_round(a.y_type, y[e]) : 0.0f;
-          amax = fmaxf(amax, finite_abs(y[e]));
+          if (!kWhole || e == 0) in = col + e < cols;
+          y[e] = in ? y[e] : 0.0f;
+          amax = fmaxf(amax, fabsf(y[e]));
         }
-        const int e8 = block_exponent(max16(amax), a.fp8);
+        amax = max16(amax);
+        if (!(amax < __builtin_inff())) {  // infinities do not count
+          amax = 0.0f;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) amax = fmaxf(amax, finite_abs(y[e]));
+          amax = max16(amax);
+        }
+        const int e8 = block_exponent(amax, a.fp8);
         if (col < blocks * 128) {
           *(uint2*)(a.q + (size_t)row * blocks * 128 + col) = quantize8(y, e8, a.fp8);
           if (t % 16 == 0) a.q_scale[(size_t)(col / 128) * a.rows + row] = (uint8_t)(e8 + 127);
@@ -189,6 +202,7 @@ extern "C" int svoo_layer_norm_fwd(const void* x, int x_type, long long x_batch_
   SVOO_REQUIRE((y != nullptr) != (q != nullptr) && (q != nullptr) == (q_scale != nullptr), SVOO_ERR_INVALID_ARG,
                "%s: one of y and (q, q_scale)", name);
   SVOO_REQUIRE((uintptr_t)q % 8 == 0, SVOO_ERR_INVALID_ARG, "%s: q must start at an 8-byte address", name);
+  SVOO_REQUIRE(q == nullptr || y_type == x_type, SVOO_ERR_UNSUPPORTED, "%s: 8-bit rows of another type than x's", name);
   SVOO_REQUIRE(x, SVOO_ERR_INVALID_ARG, "%s: null pointer", name);
   NormArgs a = {x, x_type, x_batch_stride, x_row_stride, w, b, w_batch_stride, b_batch_stride, w_type, b_type,
                 modulated ? 1.0f : 0.0f, y, y_type, q, q_scale, fp8_type, mean, rstd, (unsigned)rows,

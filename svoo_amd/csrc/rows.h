@@ -27,10 +27,19 @@ __device__ __forceinline__ void set_row_elem(void* p, int type, long long i, flo
 }
 
 // v as the row's type holds it.
-__device__ __forceinline__ float row_round(int type, float v) {
-  if (type == kRowBf16) return bf16_round_f32(v);
-  if (type == kRowF16) return (float)(_Float16)v;
-  return v;
+template <int T>
+__device__ __forceinline__ void round_row8(float (&f)[8]) {  // to the type and back
+#pragma unroll
+  for (int e = 0; e < 8; e += 2) {
+    if (T == kRowBf16) {
+      const uint32_t w = cvt_pk_bf16(f[e], f[e + 1]);
+      f[e] = __uint_as_float(w << 16);
+      f[e + 1] = __uint_as_float(w & 0xffff0000u);
+    } else if (T == kRowF16) {
+      f[e] = (float)(_Float16)f[e];
+      f[e + 1] = (float)(_Float16)f[e + 1];
+    }
+  }
 }
 
 // Elements i .. i + 7 of a row, the first n of them (n <= 0: none) and zeros.  kWhole: n is a multiple of 8.
