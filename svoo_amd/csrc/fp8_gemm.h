@@ -253,7 +253,7 @@ __device__ __forceinline__ void store_rows32(const GemmArgs& g, f32x4_t (&acc)[F
 // of bank conflicts.  A wave holds one stage's operands in registers and reads the next ones while its matrix instructions
 // run.  A barrier in the middle of a stage and one at its end each free half of a stage's place, which the copies for the
 // same half of the stage after next then fill: they have a stage's time to land, and go out evenly.  (With one barrier
-// they had half of it, in bursts that kept the waves waiting to issue: 3000 cycles a stage instead of 2400.)
+// they had half of it, in bursts that kept the waves waiting to issue: 3000 cycles a stage instead of 2500.)
 // Blocks stay, one per CU (kTile 256) or two (128), and walk over their items without a break in that sequence: the copies
 // and reads for the next tile run while the last positions of a tile are multiplied.
 // The matrix instruction's first operand is b and its second a: a lane then holds four consecutive columns of a row of c.
