@@ -163,11 +163,12 @@ static void for_type(int type, F f) {
   else f(std::integral_constant<int, kRowF32>());
 }
 
-// Blocks that share a batch entry's rows in the backward pass: two per CU in all, and no fewer than four rows a group
-// where there are more.
+// Blocks that share a batch entry's rows in the backward pass: two per CU in all, eight or four where a lane has one chunk
+// and registers for more waves, and no fewer than four rows a group where there are more.  bf16, two against eight or four:
+// 256 columns 723 and 458 us, 512 424 and 360, 2048 403 and 311; with two chunks a lane 1024 columns 301 and 349.
 static unsigned grad_parts(long long batch, long long rows_per_batch, int cols) {
   const long long groups = cols <= 128 ? 16 : cols <= 1536 ? 4 : 1;
-  const long long most = std::max(512 / batch, 1ll), want = (rows_per_batch + 4 * groups - 1) / (4 * groups);
+  const long long most = std::max((cols <= 512 ? 2048 : cols > 1536 && cols <= 2048 ? 1024 : 512) / batch, 1ll), want = (rows_per_batch + 4 * groups - 1) / (4 * groups);
   return (unsigned)std::min(most, std::max(want, 1ll));
 }
 
