@@ -23,7 +23,7 @@ from .fp8 import FP8_TYPES, empty_fp8, empty_scales
 
 def _param(p, cols: int, batch: int, device, name: str):
     """``p`` as what the C entry takes: ``(pointer, type, elements between batch entries)``, with the tensor read (kept
-    alive by the caller)."""
+    alive by the caller) and whether it has a row per batch entry.  Expanded rows are such rows too, 0 elements apart."""
     kind = _lib.elem_type(p, name)
     shape = p.shape
     if p.device != device:
@@ -34,18 +34,23 @@ def _param(p, cols: int, batch: int, device, name: str):
         raise ValueError(f"{name}: shape {tuple(shape)}; [{cols}] or [{batch}, 1, .., {cols}] expected")
     if p.stride(-1) != 1 and cols > 1:
         p = p.contiguous()
-    return p, (p.data_ptr(), kind, p.stride(0) if dims > 1 and shape[0] == batch and batch > 1 else 0)
+    each = dims > 1 and shape[0] == batch and batch > 1
+    return p, (p.data_ptr(), kind, p.stride(0) if each else 0), each
 
 
 _NO_PARAM = (None, 2, 0)
 
 
 class _Call:
-    """The checked arguments of a layer norm: x as ``[batch, rows, cols]`` by its strides, and its parameters."""
+    """The checked arguments of a layer norm: x as ``[batch, rows, cols]`` by its strides, and its parameters.
 
-    __slots__ = ("x", "x_args", "cols", "eps", "device", "shape", "batch", "rows", "modulated", "params", "args", "keep")
+    x is split by batch entries where a parameter's values differ between them, and where a gradient of a parameter with
+    a row per entry is wanted (``grads``, of the two parameters)."""
 
-    def __init__(self, x, weight, bias, scale, shift, eps):
+    __slots__ = ("x", "x_args", "cols", "eps", "device", "shape", "batch", "rows", "modulated", "params", "args", "each",
+                 "keep")
+
+    def __init__(self, x, weight, bias, scale, shift, eps, grads=(False, False)):
         self.modulated = scale is not None or shift is not None
         if self.modulated and (weight is not None or bias is not None):
             raise ValueError("layer_norm: weight and bias or scale and shift, not both")
@@ -62,15 +67,17 @@ class _Call:
             self.params, names = (scale, shift), ("scale", "shift")
         else:
             self.params, names = (weight, bias), ("weight", "bias")
-        self.keep, self.args = [], []
-        for p, name in zip(self.params, names):
-            if p is None:
-                self.args.append(_NO_PARAM)
-            else:
-                p, args = _param(p, self.cols, batch, x.device, name)
+        self.keep, self.args, self.each = [], [], []
+        split = False
+        for p, name, grad in zip(self.params, names, grads):
+            args, each = _NO_PARAM, False
+            if p is not None:
+                p, args, each = _param(p, self.cols, batch, x.device, name)
                 self.keep.append(p)
-                self.args.append(args)
-        self.batch = batch if self.args[0][2] or self.args[1][2] else 1
+                split = split or args[2] != 0 or (each and grad)
+            self.args.append(args)
+            self.each.append(each)
+        self.batch = batch if split else 1
         self.rows = x.numel() // self.cols // self.batch if self.batch else 0
         self.x_args = (*self.rows_of(x, x_type),)
 
@@ -123,7 +130,7 @@ def layer_norm_bwd(dy, x, mean, rstd, weight=None, bias=None, *, scale=None, shi
         if not isinstance(t, torch.Tensor) or t.dtype != torch.float32 or t.shape != x.shape[:-1] or t.device != x.device:
             raise ValueError(f"{name}: fp32 of shape {tuple(x.shape[:-1])} on {x.device} expected")
     mean, rstd = mean.contiguous(), rstd.contiguous()
-    return _backward(dy, _Call(x, weight, bias, scale, shift, eps), mean.data_ptr(), rstd.data_ptr(), needs)
+    return _backward(dy, _Call(x, weight, bias, scale, shift, eps, needs[1:]), mean.data_ptr(), rstd.data_ptr(), needs)
 
 
 def _backward(dy, c: _Call, mean: int, rstd: int, needs):
@@ -141,7 +148,7 @@ def _backward(dy, c: _Call, mean: int, rstd: int, needs):
     types = [2, 2]
     for i, p in enumerate(c.params):
         if want[i]:
-            own = c.args[i][2] or c.batch == 1
+            own = c.each[i] or c.batch == 1
             grads[i] = torch.empty(p.shape if own else (c.batch, c.cols), dtype=p.dtype if own else torch.float32,
                                    device=c.device)
             types[i] = _lib.elem_type(grads[i], "")
@@ -173,7 +180,8 @@ class _LayerNorm(torch.autograd.Function):
         x, p0, p1, st = ctx.saved_tensors
         params = (None, None, p0, p1) if ctx.modulated else (p0, p1, None, None)
         at = st.data_ptr()
-        grads = _backward(dy, _Call(x, *params, ctx.eps), at, at + 4 * st.shape[1], ctx.needs_input_grad)
+        needs = ctx.needs_input_grad[:3]
+        grads = _backward(dy, _Call(x, *params, ctx.eps, needs[1:]), at, at + 4 * st.shape[1], needs)
         return (*grads, None, None, None)
 
 
