@@ -173,8 +173,51 @@ def elem_type(t: torch.Tensor, name: str) -> int:
     return _ELEM_TYPES[t.dtype]
 
 
+def _recorder() -> Optional[str]:
+    """What records the tensor operations of this moment, if anything does.  Some of these can only be asked of names that
+    torch keeps to itself: without them only ``torch.jit.trace`` is known."""
+    if torch.jit.is_tracing():
+        return "torch.jit.trace"
+    try:
+        # both kinds of modes are on a stack while an fx graph is made; asking for that itself takes longer
+        if torch._C._len_torch_dispatch_stack() + torch._C._len_torch_function_stack() > 0 and \
+                torch.fx.experimental.proxy_tensor.get_proxy_mode() is not None:
+            return "an fx graph's tracer"
+    except AttributeError:
+        pass
+    return None
+
+
+def _has_tangent(t) -> bool:
+    return isinstance(t, torch.Tensor) and torch.autograd.forward_ad.unpack_dual(t).tangent is not None
+
+
+def refuse_unseen(name: str, *tensors) -> None:
+    """A kernel launched on raw pointers appears in no record of tensor operations, which would keep the allocation of its
+    result alone, and carries no tangents: refused while such a record is made and for tensors with tangents."""
+    by = _recorder()
+    if by is not None:
+        raise RuntimeError(f"{name} cannot be recorded by {by}")
+    if getattr(torch.autograd.forward_ad, "_current_level", 0) >= 0 and any(_has_tangent(t) for t in tensors):
+        raise RuntimeError(f"{name} has no forward-mode derivative: call it on tensors without tangents")
+
+
+def traced_or_transformed() -> bool:
+    """A program between operators may be recorded, transformed or carry tangents: launches on raw pointers would be
+    refused or lost where tensor operations are not."""
+    if _recorder() is not None:
+        return True
+    try:
+        return torch.autograd.forward_ad._current_level >= 0 or \
+            torch._C._functorch.peek_interpreter_stack() is not None
+    except AttributeError:
+        return False
+
+
 def refuse_grad(name: str, *tensors) -> None:
-    """An operator without a backward pass takes no tensor that waits for a gradient: its result would end the graph."""
+    """An operator without a backward pass takes no tensor that waits for a gradient: its result would end the graph.
+    :func:`refuse_unseen` besides."""
+    refuse_unseen(name, *tensors)
     if not torch.is_grad_enabled():
         return
     if any(t is not None and t.requires_grad for t in tensors):

@@ -20,7 +20,7 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
-from . import norm
+from . import _lib, norm
 from .fp8 import Fp8Linear
 
 
@@ -117,8 +117,8 @@ class WanBlock(nn.Module):
     """One Wan DiT block: modulated self-attention, cross-attention to the text, modulated FFN.
 
     With ``fused_norms`` each norm and its modulation are one pass (:func:`svoo_amd.norm.layer_norm`, differentiable) in
-    place of the norm modules' calls, and an 8-bit FFN (:func:`svoo_amd.inference.replace_wan_linear`) takes its input as
-    8-bit rows from the norm."""
+    place of the norm modules' calls (which stay where the block is traced, transformed or under forward-mode AD), and an
+    8-bit FFN (:func:`svoo_amd.inference.replace_wan_linear`) takes its input as 8-bit rows from the norm."""
 
     fused_norms = False
 
@@ -138,24 +138,25 @@ class WanBlock(nn.Module):
         mod = (self.scale_shift_table.float() + temb.float()).chunk(6, dim=1)
         shift, scale, gate, c_shift, c_scale, c_gate = mod
         dtype = hidden_states.dtype
-        if self.fused_norms:
+        fused = self.fused_norms and not _lib.traced_or_transformed()
+        if fused:
             x = norm.layer_norm(hidden_states, scale=scale, shift=shift, eps=self.norm1.eps)
         else:
             x = (self.norm1(hidden_states.float()) * (1 + scale) + shift).to(dtype)
         a = self.attn1(hidden_states=x, rotary_emb=rotary_emb, timestep=timestep)
         hidden_states = (hidden_states.float() + a.float() * gate).to(dtype)
-        if self.fused_norms:
+        if fused:
             x = norm.layer_norm(hidden_states, self.norm2.weight, self.norm2.bias, eps=self.norm2.eps)
         else:
             x = self.norm2(hidden_states.float()).to(dtype)
         hidden_states = hidden_states + self.attn2(hidden_states=x, encoder_hidden_states=encoder_hidden_states)
-        if self.fused_norms and isinstance(self.ffn[0], Fp8Linear) and not _watched(self.ffn, self.ffn[0]):
+        if fused and isinstance(self.ffn[0], Fp8Linear) and not _watched(self.ffn, self.ffn[0]):
             rows = norm.layer_norm_fp8(hidden_states, scale=c_scale, shift=c_shift, eps=self.norm3.eps)
             first, *rest = self.ffn
             f = first.forward_quantized(*rows, out_dtype=dtype)
             for layer in rest:
                 f = layer(f)
-        elif self.fused_norms:
+        elif fused:
             f = self.ffn(norm.layer_norm(hidden_states, scale=c_scale, shift=c_shift, eps=self.norm3.eps))
         else:
             x = (self.norm3(hidden_states.float()) * (1 + c_scale) + c_shift).to(dtype)
@@ -235,7 +236,7 @@ class WanDiT(nn.Module):
         for block in self.blocks:
             x = block(x, ctx, tproj, rotary, timestep=timestep)
         shift, scale = (self.scale_shift_table.float() + temb.float()[:, None]).chunk(2, dim=1)
-        if self.fused_norms:
+        if self.fused_norms and not _lib.traced_or_transformed():
             x = norm.layer_norm(x, scale=scale, shift=shift, eps=self.norm_out.eps)
         else:
             x = (self.norm_out(x.float()) * (1 + scale) + shift).to(x.dtype)

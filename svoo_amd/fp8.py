@@ -175,6 +175,7 @@ class _Operand:
 def fp8_dequantize(q: torch.Tensor, s: torch.Tensor, cols: Optional[int] = None, out_dtype=torch.bfloat16) -> torch.Tensor:
     """The values ``[.., cols]`` (all stored columns by default) that 8-bit values and their scales stand for, rounded to
     ``out_dtype``.  ``s`` has a row for each row of q, or for each 128 of a matrix's rows."""
+    _lib.refuse_unseen("fp8_dequantize", q)
     o = _Operand(q, s, "q", _BOTH, True)
     cols = o.kp if cols is None else int(cols)
     if not o.kp - BLOCK < cols <= o.kp:
@@ -262,6 +263,7 @@ def fp8_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tenso
     fp32 sums of the unquantised gradient.  Results have the type of x, of weight and of bias.
 
     Kept for the backward pass: 8-bit copies of x and of the weight."""
+    _lib.refuse_unseen("fp8_linear", x, weight, bias)
     _fp8_type(grad_dtype, "fp8_linear")
     _lib.elem_type(weight, "weight")
     if weight.dim() != 2 or 0 in weight.shape or x.dim() == 0 or x.shape[-1] != weight.shape[1] or \

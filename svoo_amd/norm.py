@@ -126,6 +126,7 @@ def layer_norm_bwd(dy, x, mean, rstd, weight=None, bias=None, *, scale=None, shi
 
     Pass the parameters the forward pass had: a gradient has its parameter's shape and type and is None without one, or
     where ``needs`` says so.  Sums over rows are fp32 in a fixed order: the same call gives the same bits."""
+    _lib.refuse_unseen("layer_norm_bwd", dy, x, mean, rstd, weight, bias, scale, shift)
     for t, name in ((mean, "mean"), (rstd, "rstd")):
         if not isinstance(t, torch.Tensor) or t.dtype != torch.float32 or t.shape != x.shape[:-1] or t.device != x.device:
             raise ValueError(f"{name}: fp32 of shape {tuple(x.shape[:-1])} on {x.device} expected")
@@ -194,6 +195,7 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
     Parameters are ``[C]``, or ``[B, C]`` / ``[B, 1, .., C]`` with one row for each entry of x's first dimension
     (modulation vectors; strided ones are read in place).  Types may differ from x's.  The result has ``out_dtype``
     (x's by default).  Differentiable in x and the parameters, once."""
+    _lib.refuse_unseen("layer_norm", x, weight, bias, scale, shift)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, scale, shift)):
         modulated = scale is not None or shift is not None
         if modulated and (weight is not None or bias is not None):

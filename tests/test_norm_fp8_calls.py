@@ -74,3 +74,119 @@ def test_forward_reads_expanded_parameters_as_shared_ones(launches):
     (_, fwd), (_, bwd) = launches
     assert fwd[12:15] == (1, 28, 16)
     assert dict(zip(BWD, bwd))["batch"] == 1
+
+
+# ------------------------------------------------------------------------------------------------ records and tangents
+def _operators():
+    """Every operator as a function of one matrix, by name."""
+    from svoo_amd import fp8, norm
+
+    w, st = torch.randn(128, 128), torch.zeros(4)
+    a, b = fp8.fp8_quantize_rows(w), fp8.fp8_quantize_blocks(w)
+    train = fp8.Fp8TrainLinear(128, 128)
+    return {
+        "layer_norm": lambda x: norm.layer_norm(x), "layer_norm of a scale": lambda x: norm.layer_norm(w[:4], scale=x),
+        "layer_norm_fwd": lambda x: norm.layer_norm_fwd(x)[0], "layer_norm_fp8": lambda x: norm.layer_norm_fp8(x)[0],
+        "layer_norm_bwd": lambda x: norm.layer_norm_bwd(x, w[:4], st, st)[0],
+        "layer_norm_bwd of x": lambda x: norm.layer_norm_bwd(w[:4], x, st, st)[0],
+        "fp8_quantize_rows": lambda x: fp8.fp8_quantize_rows(x)[0],
+        "fp8_quantize_blocks": lambda x: fp8.fp8_quantize_blocks(x)[0],
+        "fp8_quantize_both": lambda x: fp8.fp8_quantize_both(x)[0],
+        "fp8_linear": lambda x: fp8.fp8_linear(x, w), "fp8_linear of a weight": lambda x: fp8.fp8_linear(w, x),
+        "Fp8TrainLinear": train, "Fp8Linear": fp8.Fp8Linear(w),
+        "fp8_matmul of a bias": lambda x: fp8.fp8_matmul(*a, *b, x[0]),
+    }
+
+
+NAMES = ["layer_norm", "layer_norm of a scale", "layer_norm_fwd", "layer_norm_fp8", "layer_norm_bwd", "layer_norm_bwd of x",
+         "fp8_quantize_rows", "fp8_quantize_blocks", "fp8_quantize_both", "fp8_linear", "fp8_linear of a weight",
+         "Fp8TrainLinear", "Fp8Linear", "fp8_matmul of a bias"]
+
+
+@pytest.fixture
+def on_cpu(launches, monkeypatch):
+    """8-bit operands on the CPU too."""
+    from svoo_amd import fp8
+
+    monkeypatch.setattr(torch.Tensor, "is_cuda", True, raising=False)
+    monkeypatch.setattr(fp8._lib, "workspace", lambda n, device: torch.empty(max(n, 1), dtype=torch.uint8))
+    return launches
+
+
+@pytest.mark.parametrize("name", NAMES)
+@pytest.mark.parametrize("grad", [False, True])
+def test_tangents_are_refused(on_cpu, name, grad):
+    """A tensor with a tangent would come out without one; in the same level, tensors without tangents are taken."""
+    import torch.autograd.forward_ad as fwd
+
+    with torch.set_grad_enabled(grad):
+        f = _operators()[name]
+        x = torch.randn(4, 128)
+        on_cpu.clear()
+        with fwd.dual_level():
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                f(fwd.make_dual(x, torch.ones_like(x)))
+            assert not on_cpu
+            if name != "Fp8TrainLinear" or not grad:
+                f(x)
+                assert on_cpu
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_tracing_is_refused(on_cpu, name):
+    """A trace would hold the allocation of the result and no launch: refused by name, before one."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    f = _operators()[name]
+    x = torch.randn(4, 128)
+    on_cpu.clear()
+    with torch.no_grad():
+        with pytest.raises(RuntimeError, match="cannot be recorded"):
+            torch.jit.trace(f, (x,), check_trace=False)
+        for pre_dispatch in (False, True):
+            with pytest.raises(RuntimeError, match="cannot be recorded"):
+                make_fx(f, pre_dispatch=pre_dispatch)(x)
+        assert not on_cpu
+        with torch.device("cpu"):  # a function mode that records nothing
+            f(x)
+        assert on_cpu
+
+
+class _Mix:
+    def __call__(self, attn, hidden_states, encoder_hidden_states=None, attention_mask=None, rotary_emb=None, timestep=None):
+        return attn.to_out[0](attn.to_q(hidden_states))
+
+
+def _block():
+    from svoo_amd import dit
+
+    torch.manual_seed(0)
+    cfg = dit.WanDiTConfig(num_attention_heads=1, ffn_dim=64, num_layers=1, text_dim=32)
+    block = dit.make_pipe(cfg, dtype=torch.float32).transformer.blocks[0].requires_grad_(False)
+    for attn in (block.attn1, block.attn2):
+        attn.set_processor(_Mix())
+    return block, torch.randn(1, 5, cfg.dim), torch.randn(1, 3, cfg.dim), torch.randn(1, 6, cfg.dim)
+
+
+def test_fused_norms_step_back_for_records_and_tangents(launches):
+    """A block with fused norms traces and takes tangents as one without."""
+    import torch.autograd.forward_ad as fwd
+
+    block, x, ctx, temb = _block()
+
+    def run(x):
+        return block(x, ctx, temb, None)
+
+    def tangent():
+        with fwd.dual_level():
+            return fwd.unpack_dual(run(fwd.make_dual(x, torch.ones_like(x)))).tangent
+
+    with torch.no_grad():
+        want, want_traced = tangent(), torch.jit.trace(run, (x,), check_trace=False)(2 * x)
+        block.fused_norms = True
+        assert torch.equal(tangent(), want)
+        assert torch.equal(torch.func.jvp(run, (x,), (torch.ones_like(x),))[1], want)
+        assert torch.equal(torch.jit.trace(run, (x,), check_trace=False)(2 * x), want_traced)
+        assert not launches
+        run(x)
+        assert [name for name, _ in launches] == ["svoo_layer_norm_fwd"] * 3
