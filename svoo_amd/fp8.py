@@ -215,21 +215,27 @@ def fp8_matmul(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale:
     return c
 
 
+def _linear(x, weight, bias, need_x: bool, need_w: bool):
+    """``(y, (wqt, wst, qt, st))``: the layer's output, and the transposed weight and rows that the gradients of x and of
+    the weight will read (None where they will not)."""
+    rows, kind = _matrix(x, "x")
+    w, w_kind = _matrix(weight, "weight")
+    wq, ws, wqt, wst = _tiles(w, w_kind, torch.float8_e4m3fn, True, True, need_x)
+    if need_w:
+        q, s, qt, st = _tiles(rows, kind, torch.float8_e4m3fn, False, True, True)
+    else:
+        (q, s), qt, st = fp8_quantize_rows(rows), None, None
+    y = fp8_matmul(q, s, wq, ws, bias, out_dtype=x.dtype)
+    return y.view(*x.shape[:-1], w.shape[0]), (wqt, wst, qt, st)
+
+
 class _Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, grad_dtype):
-        rows, kind = _matrix(x, "x")
-        w, w_kind = _matrix(weight, "weight")
-        need_x, need_w = ctx.needs_input_grad[:2]
-        wq, ws, wqt, wst = _tiles(w, w_kind, torch.float8_e4m3fn, True, True, need_x)
-        if need_w:
-            q, s, qt, st = _tiles(rows, kind, torch.float8_e4m3fn, False, True, True)
-        else:
-            (q, s), qt, st = fp8_quantize_rows(rows), None, None
-        y = fp8_matmul(q, s, wq, ws, bias, out_dtype=x.dtype)
-        ctx.save_for_backward(wqt, wst, qt, st)
+        y, kept = _linear(x, weight, bias, *ctx.needs_input_grad[:2])
+        ctx.save_for_backward(*kept)
         ctx.meta = x.shape, x.dtype, weight.shape, weight.dtype, None if bias is None else bias.dtype, grad_dtype
-        return y.view(*x.shape[:-1], w.shape[0])
+        return y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
@@ -262,14 +268,16 @@ def fp8_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tenso
     of a wide range) and the weight, ``dweight`` from the gradient's and x's columns in blocks of 128 rows, ``dbias`` in
     fp32 sums of the unquantised gradient.  Results have the type of x, of weight and of bias.
 
-    Kept for the backward pass: 8-bit copies of x and of the weight."""
+    Kept for the backward pass: 8-bit copies of x and of the weight (not made where no gradient can be asked for)."""
     _lib.refuse_unseen("fp8_linear", x, weight, bias)
     _fp8_type(grad_dtype, "fp8_linear")
     _lib.elem_type(weight, "weight")
     if weight.dim() != 2 or 0 in weight.shape or x.dim() == 0 or x.shape[-1] != weight.shape[1] or \
             weight.device != x.device:
         raise ValueError(f"fp8_linear: x {tuple(x.shape)} on {x.device}, weight {tuple(weight.shape)} on {weight.device}")
-    return _Linear.apply(x, weight, bias, grad_dtype)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
+        return _Linear.apply(x, weight, bias, grad_dtype)
+    return _linear(x, weight, bias, False, False)[0]
 
 
 class Fp8Linear(torch.nn.Module):

@@ -190,3 +190,26 @@ def test_fused_norms_step_back_for_records_and_tangents(launches):
         assert not launches
         run(x)
         assert [name for name, _ in launches] == ["svoo_layer_norm_fwd"] * 3
+
+
+# ------------------------------------------------------------------------------------------------ no work for a backward pass
+@pytest.mark.parametrize("how", ["no_grad", "inference_mode", "nothing requires a gradient", "x alone", "weight alone", "both"])
+def test_linear_lays_out_what_its_backward_pass_reads_and_no_more(on_cpu, how):
+    """Transposed copies of the weight (for dx) and of x (for dw) where that gradient may be asked for; none in evaluation."""
+    import contextlib
+
+    from svoo_amd import fp8
+
+    off = {"no_grad": torch.no_grad, "inference_mode": torch.inference_mode}.get(how)
+    x = torch.randn(3, 5, 64, requires_grad=off is not None or how in ("x alone", "both"))
+    w = torch.randn(32, 64, requires_grad=off is not None or how in ("weight alone", "both"))
+    with off() if off is not None else contextlib.nullcontext():
+        y = fp8.fp8_linear(x, w, torch.randn(32, requires_grad=off is not None))
+    need_x, need_w = how in ("x alone", "both"), how in ("weight alone", "both")
+    assert y.shape == (3, 5, 32) and y.requires_grad == (need_x or need_w)
+    names, args = zip(*on_cpu)
+    assert names == ("svoo_fp8_quantize_tiles", "svoo_fp8_quantize_tiles" if need_w else "svoo_fp8_quantize_rows",
+                     "svoo_fp8_matmul")
+    assert (args[0][9] is not None) == need_x  # the weight's transposed values
+    if need_w:
+        assert args[1][9] is not None
