@@ -55,9 +55,10 @@ __device__ __forceinline__ void norm_rows(const NormArgs& a, const f32x4_t* w, c
     }
     row_sums<TPR>(d1, d2, scratch, half);
     // what the rounding of the mean left over: the deviations' own mean
-    const float dm = d1 * inv, rstd = 1.0f / sqrtf(fmaxf(fmaf(-dm, dm, d2 * inv), 0.0f) + a.eps);
+    const float dm = d1 * inv, var = fmaf(-dm, dm, d2 * inv);
+    const float rstd = 1.0f / sqrtf((var < 0.0f ? 0.0f : var) + a.eps);  // NaN stays
     if (t == 0) {
-      if (a.mean != nullptr) a.mean[row] = mean0 + dm;
+      if (a.mean != nullptr) a.mean[row] = fabsf(mean0) < __builtin_inff() ? mean0 + dm : mean0;
       if (a.rstd != nullptr) a.rstd[row] = rstd;
     }
     x.forget();
