@@ -34,6 +34,7 @@ from .sparsity.exact import (compute_exact_attention_sparsity, format_sparsity_l
                              record_sparsity_entry)
 from .permute import apply_inverse_permutation, apply_inverse_permutation_bshd, permute_pair_by_indices
 from . import _lib, heads
+from .fp8 import Fp8TrainLinear
 
 
 def _env_on(name: str) -> bool:
@@ -84,6 +85,15 @@ def _apply_rotary_emb(hidden_states: torch.Tensor, freqs_cos: torch.Tensor, freq
     out[..., 0::2] = x1 * cos - x2 * sin
     out[..., 1::2] = x1 * sin + x2 * cos
     return out.type_as(hidden_states)
+
+
+def _refuse_lost_gradients(attn, qkv, out) -> None:
+    """8-bit projections that exist to train (:class:`svoo_amd.fp8.Fp8TrainLinear`) would get no gradient through the
+    sparse kernels, and no error either."""
+    if torch.is_grad_enabled() and not out.requires_grad and any(t.requires_grad for t in qkv) and \
+            any(isinstance(getattr(attn, n, None), Fp8TrainLinear) for n in ("to_q", "to_k", "to_v")):
+        raise RuntimeError("sparse attention has no backward pass: trainable 8-bit projections would get no gradient "
+                           "through it (run it under torch.no_grad(), or train with dense attention)")
 
 
 class WanAttn_SAPAttn_Processor:
@@ -274,6 +284,7 @@ class WanAttn_SAPAttn_Processor:
             if self.measure_attention_sparsity:
                 self.log_attention_sparsity(query, key, value, timestep, "self")
             hidden_states = self.attention_core_logic(query, key, value, timestep)
+            _refuse_lost_gradients(attn, (query, key, value), hidden_states)
         return self.get_o(attn, query, hidden_states, hidden_states_img)
 
     # ---------------------------------------------------------------- step bookkeeping

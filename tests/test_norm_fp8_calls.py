@@ -103,53 +103,43 @@ NAMES = ["layer_norm", "layer_norm of a scale", "layer_norm_fwd", "layer_norm_fp
          "Fp8TrainLinear", "Fp8Linear", "fp8_matmul of a bias"]
 
 
-@pytest.fixture
-def on_cpu(launches, monkeypatch):
-    """8-bit operands on the CPU too."""
-    from svoo_amd import fp8
-
-    monkeypatch.setattr(torch.Tensor, "is_cuda", True, raising=False)
-    monkeypatch.setattr(fp8._lib, "workspace", lambda n, device: torch.empty(max(n, 1), dtype=torch.uint8))
-    return launches
-
-
 @pytest.mark.parametrize("name", NAMES)
 @pytest.mark.parametrize("grad", [False, True])
-def test_tangents_are_refused(on_cpu, name, grad):
+def test_tangents_are_refused(launches, name, grad):
     """A tensor with a tangent would come out without one; in the same level, tensors without tangents are taken."""
     import torch.autograd.forward_ad as fwd
 
     with torch.set_grad_enabled(grad):
         f = _operators()[name]
         x = torch.randn(4, 128)
-        on_cpu.clear()
+        launches.clear()
         with fwd.dual_level():
             with pytest.raises(RuntimeError, match="forward-mode"):
                 f(fwd.make_dual(x, torch.ones_like(x)))
-            assert not on_cpu
+            assert not launches
             if name != "Fp8TrainLinear" or not grad:
                 f(x)
-                assert on_cpu
+                assert launches
 
 
 @pytest.mark.parametrize("name", NAMES)
-def test_tracing_is_refused(on_cpu, name):
+def test_tracing_is_refused(launches, name):
     """A trace would hold the allocation of the result and no launch: refused by name, before one."""
     from torch.fx.experimental.proxy_tensor import make_fx
 
     f = _operators()[name]
     x = torch.randn(4, 128)
-    on_cpu.clear()
+    launches.clear()
     with torch.no_grad():
         with pytest.raises(RuntimeError, match="cannot be recorded"):
             torch.jit.trace(f, (x,), check_trace=False)
         for pre_dispatch in (False, True):
             with pytest.raises(RuntimeError, match="cannot be recorded"):
                 make_fx(f, pre_dispatch=pre_dispatch)(x)
-        assert not on_cpu
+        assert not launches
         with torch.device("cpu"):  # a function mode that records nothing
             f(x)
-        assert on_cpu
+        assert launches
 
 
 class _Mix:
@@ -194,7 +184,7 @@ def test_fused_norms_step_back_for_records_and_tangents(launches):
 
 # ------------------------------------------------------------------------------------------------ no work for a backward pass
 @pytest.mark.parametrize("how", ["no_grad", "inference_mode", "nothing requires a gradient", "x alone", "weight alone", "both"])
-def test_linear_lays_out_what_its_backward_pass_reads_and_no_more(on_cpu, how):
+def test_linear_lays_out_what_its_backward_pass_reads_and_no_more(launches, how):
     """Transposed copies of the weight (for dx) and of x (for dw) where that gradient may be asked for; none in evaluation."""
     import contextlib
 
@@ -207,9 +197,37 @@ def test_linear_lays_out_what_its_backward_pass_reads_and_no_more(on_cpu, how):
         y = fp8.fp8_linear(x, w, torch.randn(32, requires_grad=off is not None))
     need_x, need_w = how in ("x alone", "both"), how in ("weight alone", "both")
     assert y.shape == (3, 5, 32) and y.requires_grad == (need_x or need_w)
-    names, args = zip(*on_cpu)
+    names, args = zip(*launches)
     assert names == ("svoo_fp8_quantize_tiles", "svoo_fp8_quantize_tiles" if need_w else "svoo_fp8_quantize_rows",
                      "svoo_fp8_matmul")
     assert (args[0][9] is not None) == need_x  # the weight's transposed values
     if need_w:
         assert args[1][9] is not None
+
+
+# ------------------------------------------------------------------------------------------------ training beside attention
+@pytest.mark.parametrize("lost", [False, True])
+@pytest.mark.parametrize("trainable", [False, True])
+def test_attention_without_a_backward_pass_refuses_trainable_8_bit_projections(launches, lost, trainable):
+    """A result without a graph from projections with one is refused for the layers that exist to train, and only there."""
+    from types import SimpleNamespace
+
+    from svoo_amd import fp8
+    from svoo_amd.processor import WanAttn_SAPAttn_Processor
+
+    class Processor(WanAttn_SAPAttn_Processor):
+        def attention_core_logic(self, query, key, value, timestep):
+            out = (query + key + value).transpose(1, 2).flatten(2, 3)
+            return out.detach() if lost else out
+
+    make = fp8.Fp8TrainLinear if trainable else torch.nn.Linear
+    attn = SimpleNamespace(heads=1, to_q=make(64, 64), to_k=make(64, 64), to_v=make(64, 64), to_out=[lambda t: t] * 2)
+    proc, x, t = Processor(0), torch.randn(1, 6, 64), torch.tensor([3.0])
+    launches.clear()
+    if trainable and lost:
+        with pytest.raises(RuntimeError, match="sparse attention has no backward pass"):
+            proc(attn, x, timestep=t)
+    else:
+        assert proc(attn, x, timestep=t).requires_grad == (not lost)
+    with torch.no_grad():
+        assert proc(attn, x, timestep=t).shape == x.shape
