@@ -112,7 +112,7 @@ template <int kAt>
 __device__ __forceinline__ void buffer_dma16(i32x4_t buffer, uint32_t voff, uint32_t soff, uint32_t lds) {
   __asm__ volatile("s_add_u32 m0, %2, %4\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, %3 offen lds" ::"v"(voff), "s"(buffer),
                    "s"(lds), "s"(soff), "i"(kAt)
-                   : "memory", "scc");
+                   : "memory", "m0", "scc");
 }
 // An element of 1, 2 or 4 bytes per lane to words of LDS.
 template <int kBytes, int kAt>
@@ -120,15 +120,15 @@ __device__ __forceinline__ void buffer_dma_words(i32x4_t buffer, uint32_t voff, 
   if constexpr (kBytes == 1)
     __asm__ volatile("s_add_u32 m0, %2, %3\n\ts_nop 0\n\tbuffer_load_ubyte %0, %1, 0 offen lds" ::"v"(voff), "s"(buffer),
                      "s"(lds), "i"(kAt)
-                     : "memory", "scc");
+                     : "memory", "m0", "scc");
   else if constexpr (kBytes == 2)
     __asm__ volatile("s_add_u32 m0, %2, %3\n\ts_nop 0\n\tbuffer_load_ushort %0, %1, 0 offen lds" ::"v"(voff), "s"(buffer),
                      "s"(lds), "i"(kAt)
-                     : "memory", "scc");
+                     : "memory", "m0", "scc");
   else
     __asm__ volatile("s_add_u32 m0, %2, %3\n\ts_nop 0\n\tbuffer_load_dword %0, %1, 0 offen lds" ::"v"(voff), "s"(buffer),
                      "s"(lds), "i"(kAt)
-                     : "memory", "scc");
+                     : "memory", "m0", "scc");
 }
 template <class T>
 __device__ __forceinline__ const __attribute__((address_space(3))) T* lds_at(uint32_t at) {
