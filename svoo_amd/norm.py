@@ -134,6 +134,28 @@ def layer_norm_bwd(dy, x, mean, rstd, weight=None, bias=None, *, scale=None, shi
     return _backward(dy, _Call(x, weight, bias, scale, shift, eps, needs[1:]), mean.data_ptr(), rstd.data_ptr(), needs)
 
 
+def _launch_backward(device, x_args, dy_args, w_args, modulated, mean, rstd, batch, rows, cols, dx, grads, types):
+    ws, size = None, 0
+    if grads[0] is not None or grads[1] is not None:
+        size = _lib.lib().svoo_layer_norm_bwd_workspace_size(batch, rows, cols)
+        if size:
+            ws = _lib.workspace(size, device)
+    _lib.launch(device, "svoo_layer_norm_bwd", *x_args, *dy_args, *w_args, modulated, mean, rstd, batch, rows, cols,
+                _lib.ptr(dx), _lib.ptr(grads[0]), types[0], _lib.ptr(grads[1]), types[1], _lib.ptr(ws), size)
+
+
+def _sum_of_rows(t, out):
+    """``out`` with the sum of the rows of ``t [B, cols]`` (fp32): a bias's gradient for ``dy = t``, whatever x and the
+    statistics are, so ``t`` stands for those too.  torch's ``sum`` clears its counters by a memset, which has no place in
+    a captured graph."""
+    rows, cols = t.shape
+    at = t.data_ptr()
+    args = (at, 2, rows * cols, cols)
+    _launch_backward(t.device, args, args, _NO_PARAM, False, at, at, 1, rows, cols, None, (None, out),
+                     (2, _lib.elem_type(out, "")))
+    return out
+
+
 def _backward(dy, c: _Call, mean: int, rstd: int, needs):
     x = c.x
     dy_type = _lib.elem_type(dy, "dy")
@@ -153,16 +175,11 @@ def _backward(dy, c: _Call, mean: int, rstd: int, needs):
             grads[i] = torch.empty(p.shape if own else (c.batch, c.cols), dtype=p.dtype if own else torch.float32,
                                    device=c.device)
             types[i] = _lib.elem_type(grads[i], "")
-    ws, size = None, 0
-    if want[0] or want[1]:
-        size = _lib.lib().svoo_layer_norm_bwd_workspace_size(c.batch, c.rows, c.cols)
-        if size:
-            ws = _lib.workspace(size, c.device)
-    _lib.launch(c.device, "svoo_layer_norm_bwd", *c.x_args, *dy_args, *c.args[0], c.modulated, mean, rstd, c.batch, c.rows,
-                c.cols, _lib.ptr(dx), _lib.ptr(grads[0]), types[0], _lib.ptr(grads[1]), types[1], _lib.ptr(ws), size)
+    _launch_backward(c.device, c.x_args, dy_args, c.args[0], c.modulated, mean, rstd, c.batch, c.rows, c.cols, dx, grads,
+                     types)
     for i, p in enumerate(c.params):
         if grads[i] is not None and grads[i].shape != p.shape:
-            grads[i] = grads[i].sum(0).to(p.dtype).view(p.shape)
+            grads[i] = _sum_of_rows(grads[i], torch.empty(p.shape, dtype=p.dtype, device=c.device))
     return dx, grads[0], grads[1]
 
 

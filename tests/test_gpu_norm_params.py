@@ -84,3 +84,58 @@ def test_gradients_of_expanded_16_bit_parameters(gpu):
     for got, p, (term, size) in zip(grads, (sc, sh), _terms(x, dy)):
         assert got.shape == p.shape and got.dtype == p.dtype
         within(got, term.sum(1), 100 * U32 * size.sum(1))
+
+
+def _memset_nodes(graph):
+    """How many nodes of a captured graph clear memory."""
+    import ctypes
+
+    hip = ctypes.CDLL("libamdhip64.so")
+    h, n = ctypes.c_void_p(graph.raw_cuda_graph()), ctypes.c_size_t()
+    assert hip.hipGraphGetNodes(h, None, ctypes.byref(n)) == 0
+    nodes = (ctypes.c_void_p * n.value)()
+    assert hip.hipGraphGetNodes(h, nodes, ctypes.byref(n)) == 0
+    count = 0
+    for node in nodes:
+        kind = ctypes.c_int()
+        assert hip.hipGraphNodeGetType(ctypes.c_void_p(node), ctypes.byref(kind)) == 0
+        count += kind.value == 2  # hipGraphNodeTypeMemset
+    return count
+
+
+@pytest.mark.parametrize("batch,rows,cols", [(3, 21, 136), (3000, 2, 64), (20000, 1, 9), (700, 3, 1536)])
+def test_shared_gradients_in_a_graph(gpu, batch, rows, cols):
+    """A parameter shared by many entries beside one that is not, captured: only kernels, and every replay is the eager
+    result, with eager work between."""
+    from svoo_amd import norm
+
+    g = torch.Generator(device=gpu).manual_seed(batch)
+    draw = lambda *s: torch.randn(*s, generator=g, device=gpu)  # noqa: E731
+    data = [(draw(batch, rows, cols).to(BF16), draw(batch, rows, cols).to(BF16), 0.3 * draw(batch, 1, cols), 0.3 * draw(cols))
+            for _ in range(2)]
+
+    def step(x, dy, sc, sh):
+        y, mean, rstd = norm.layer_norm_fwd(x, scale=sc, shift=sh)
+        return (y, *norm.layer_norm_bwd(dy, x, mean, rstd, scale=sc, shift=sh))
+
+    say("shared gradients in a graph", batch, rows, cols)
+    want = [step(*d) for d in data]
+    for (x, dy, _, _), (_, _, dsc, dsh) in zip(data, want):
+        (term, size), (d, d_size) = _terms(x, dy)
+        within(dsc.view(batch, cols), term.sum(1), (80 + rows) * U32 * size.sum(1))
+        within(dsh, d.sum((0, 1)), (80 + rows + batch) * U32 * d_size.sum((0, 1)))
+    held = [t.clone() for t in data[0]]
+    step(*held)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph(keep_graph=True)
+    with torch.cuda.graph(graph):
+        out = step(*held)
+    assert _memset_nodes(graph) == 0
+    graph.instantiate()
+    for i in range(4):
+        for h, t in zip(held, data[i % 2]):
+            h.copy_(t)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, want[i % 2])), i
+        assert all(torch.equal(a, b) for a, b in zip(step(*data[1]), want[1]))

@@ -63,6 +63,34 @@ def test_gradients_of_every_parameter_form_are_written_whole(launches, kinds, dt
             assert a[key + "_type"] == ELEM_TYPES[dtype]
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_sums_over_the_batch_are_launches_too(launches, dtype):
+    """The gradient of a parameter shared by the entries, beside one that is not: a second launch adds the entries' sums, in
+    the parameter's type, and no tensor operation (whose scratch a captured graph would clear by a memset)."""
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    from svoo_amd import norm
+
+    class Ops(TorchDispatchMode):
+        seen = []
+
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            self.seen.append(func.overloadpacket.__name__)
+            return func(*args, **(kwargs or {}))
+
+    x, st = torch.randn(6, 5, 16), torch.zeros(6, 5)
+    sc, sh = _params(6, 16, "own"), _params(6, 16, "shared", dtype)
+    with Ops() as ops:
+        _, dsc, dsh = norm.layer_norm_bwd(x, x, st, st, scale=sc, shift=sh)
+    first, second = (dict(zip(BWD, args)) for _, args in launches)
+    assert first["batch"] == 6 and first["dw"] == dsc.data_ptr() and first["db_type"] == 2
+    assert second["dy"] == first["db"] and (second["batch"], second["rows"], second["cols"]) == (1, 6, 16)
+    assert (second["dy_type"], second["dy_row"]) == (2, 16) and second["dx"] is None and second["dw"] is None
+    assert second["db"] == dsh.data_ptr() and second["db_type"] == ELEM_TYPES[dtype]
+    assert dsh.shape == (16,) and dsh.dtype == dtype and dsc.shape == (6, 1, 16)
+    assert "sum" not in ops.seen
+
+
 def test_forward_reads_expanded_parameters_as_shared_ones(launches):
     """No split by batch entries where none is needed: one batch of all rows."""
     from svoo_amd import norm
