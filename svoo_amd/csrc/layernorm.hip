@@ -181,6 +181,8 @@ static int check_norm(const char* name, int x_type, long long batch, long long r
   SVOO_REQUIRE(cols <= 16384, SVOO_ERR_UNSUPPORTED, "%s: %d columns (1..16384)", name, cols);
   SVOO_REQUIRE(batch < (1ll << 31) && rows_per_batch < (1ll << 31) && batch * rows_per_batch < (1ll << 31),
                SVOO_ERR_UNSUPPORTED, "%s: 2^31 rows or more", name);
+  // a block per batch entry at least: 1024 threads each have to fit a launch's 2^32
+  SVOO_REQUIRE(batch < (1ll << 22), SVOO_ERR_UNSUPPORTED, "%s: %lld batch entries (fewer than 2^22)", name, batch);
   return SVOO_OK;
 }
 

@@ -259,3 +259,17 @@ def test_attention_without_a_backward_pass_refuses_trainable_8_bit_projections(l
         assert proc(attn, x, timestep=t).requires_grad == (not lost)
     with torch.no_grad():
         assert proc(attn, x, timestep=t).shape == x.shape
+
+
+# ------------------------------------------------------------------------------------------------ what no launch can hold
+def test_more_batch_entries_than_a_launch_has_blocks_are_refused():
+    from svoo_amd import _lib
+
+    lib = _lib.lib()
+    for batch in (1 << 22, 1 << 30):
+        assert lib.svoo_layer_norm_fwd(16, 0, 8, 8, 16, 2, 8, None, 2, 0, 1, 1e-6, batch, 1, 8, 16, 0, None, None, 0, None,
+                                       None, None) == -2
+        assert f"{batch} batch entries" in _lib.last_error()
+        assert lib.svoo_layer_norm_bwd(16, 0, 8, 8, 16, 0, 8, 8, None, 2, 0, 1, 16, 16, batch, 1, 8, 16, 16, 2, 16, 2, None, 0,
+                                       None) == -2
+        assert f"{batch} batch entries" in _lib.last_error()
