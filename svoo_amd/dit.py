@@ -20,7 +20,7 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
-from . import _lib, norm
+from . import _lib, heads, norm
 from .fp8 import Fp8Linear
 
 
@@ -109,8 +109,9 @@ class WanAttention(nn.Module):
 
 
 def _watched(*modules) -> bool:
-    """Hooks wait for a call of one of the modules."""
-    return any(m._forward_hooks or m._forward_pre_hooks or m._backward_hooks or m._backward_pre_hooks for m in modules)
+    """Something waits for a call of one of the modules: hooks, its own or every module's, or a forward set on it."""
+    return any(getattr(nn.modules.module, n, None) for n in heads.GLOBAL_HOOKS) or \
+        any("forward" in m.__dict__ or any(getattr(m, n) for n in heads.MODULE_HOOKS) for m in modules)
 
 
 class WanBlock(nn.Module):
@@ -150,7 +151,8 @@ class WanBlock(nn.Module):
         else:
             x = self.norm2(hidden_states.float()).to(dtype)
         hidden_states = hidden_states + self.attn2(hidden_states=x, encoder_hidden_states=encoder_hidden_states)
-        if fused and isinstance(self.ffn[0], Fp8Linear) and not _watched(self.ffn, self.ffn[0]):
+        if fused and type(self.ffn) is nn.Sequential and type(self.ffn[0]) is Fp8Linear and \
+                not _watched(self.ffn, self.ffn[0]):
             rows = norm.layer_norm_fp8(hidden_states, scale=c_scale, shift=c_shift, eps=self.norm3.eps)
             first, *rest = self.ffn
             f = first.forward_quantized(*rows, out_dtype=dtype)

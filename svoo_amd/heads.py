@@ -15,9 +15,9 @@ import torch
 
 from . import _lib
 
-_GLOBAL_HOOKS = ("_global_forward_hooks", "_global_forward_pre_hooks", "_global_backward_hooks",
+GLOBAL_HOOKS = ("_global_forward_hooks", "_global_forward_pre_hooks", "_global_backward_hooks",
                  "_global_backward_pre_hooks")
-_MODULE_HOOKS = ("_forward_hooks", "_forward_pre_hooks", "_backward_hooks", "_backward_pre_hooks")
+MODULE_HOOKS = ("_forward_hooks", "_forward_pre_hooks", "_backward_hooks", "_backward_pre_hooks")
 
 
 def plain_execution() -> bool:
@@ -45,8 +45,8 @@ def rms_norm_params(norm, width: int, device) -> Optional[tuple]:
     if type(norm) is not getattr(torch.nn, "RMSNorm", None) or norm.normalized_shape != (width,) or norm.eps is None:
         return None
     mod = torch.nn.modules.module
-    if "forward" in norm.__dict__ or any(getattr(mod, n, None) for n in _GLOBAL_HOOKS) or \
-            any(getattr(norm, n, None) for n in _MODULE_HOOKS):
+    if "forward" in norm.__dict__ or any(getattr(mod, n, None) for n in GLOBAL_HOOKS) or \
+            any(getattr(norm, n, None) for n in MODULE_HOOKS):
         return None
     w = norm.weight
     if w is not None and not (_plain(w, torch.bfloat16, device) and w.is_contiguous()):
@@ -69,8 +69,8 @@ def linear_ok(module, x, width: int) -> bool:
     """``module(x)`` is a plain projection whose result :func:`rows_ok` will take: a ``torch.nn.Linear`` to ``width``
     in bf16 without gradients or hooks, of ``x [1, T, C]``."""
     if type(module) is not torch.nn.Linear or module.out_features != width or "forward" in module.__dict__ or \
-            any(getattr(torch.nn.modules.module, n, None) for n in _GLOBAL_HOOKS) or \
-            any(getattr(module, n, None) for n in _MODULE_HOOKS):
+            any(getattr(torch.nn.modules.module, n, None) for n in GLOBAL_HOOKS) or \
+            any(getattr(module, n, None) for n in MODULE_HOOKS):
         return False
     return (type(x) is torch.Tensor and x.dim() == 3 and x.shape[0] == 1 and x.is_cuda
             and all(_plain(t, torch.bfloat16, x.device) for t in (x, module.weight, module.bias) if t is not None))

@@ -273,3 +273,48 @@ def test_more_batch_entries_than_a_launch_has_blocks_are_refused():
         assert lib.svoo_layer_norm_bwd(16, 0, 8, 8, 16, 0, 8, 8, None, 2, 0, 1, 16, 16, batch, 1, 8, 16, 16, 2, 16, 2, None, 0,
                                        None) == -2
         assert f"{batch} batch entries" in _lib.last_error()
+
+
+# ------------------------------------------------------------------------------------------------ an FFN that is someone else's
+def test_an_ffn_with_a_forward_of_its_own_is_called(launches):
+    """The block hands 8-bit rows to the FFN's first layer past its call only where nothing has replaced a call: a forward
+    set on an instance (as offloading does), a subclass's, and hooks on every module get theirs."""
+    from svoo_amd import fp8
+
+    class Own(fp8.Fp8Linear):
+        def forward(self, x):
+            seen.append("subclass")
+            return super().forward(x)
+
+    class OwnSequential(torch.nn.Sequential):
+        def forward(self, x):
+            seen.append("container")
+            return super().forward(x)
+
+    seen = []
+    block, x, ctx, temb = _block()
+    block.fused_norms = True
+    plain = torch.nn.Sequential(fp8.Fp8Linear.from_linear(block.ffn[0], "gelu_tanh"), torch.nn.Identity(),
+                                fp8.Fp8Linear.from_linear(block.ffn[2]))
+
+    def run(ffn):
+        block.ffn = ffn
+        seen.clear()
+        launches.clear()
+        with torch.no_grad():
+            block(x, ctx, temb, None)
+        return [name for name, _ in launches].count("svoo_fp8_quantize_rows")
+
+    assert run(plain) == 1 and seen == []  # the second layer's rows; the first's come from the norm
+    assert run(torch.nn.Sequential(Own.from_linear(torch.nn.Linear(128, 64)), *plain[1:])) == 2 and seen == ["subclass"]
+    assert run(OwnSequential(*plain)) == 2 and seen == ["container"]
+    forward = plain[0].forward
+    plain[0].forward = lambda t: (seen.append("instance"), forward(t))[1]
+    assert run(plain) == 2 and seen == ["instance"]
+    del plain[0].forward
+    handle = torch.nn.modules.module.register_module_forward_hook(lambda m, args, out: seen.append(m))
+    try:
+        assert run(plain) == 2 and plain in seen and plain[0] in seen
+    finally:
+        handle.remove()
+    assert run(plain) == 1
