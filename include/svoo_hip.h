@@ -313,11 +313,12 @@ int svoo_layer_norm_bwd(const void* x, int x_type, long long x_batch_stride, lon
  *     128 of ITS columns, in qt and scale_t, and optionally the column sums of x (not with `square`; needs the workspace).
  *   svoo_fp8_dequantize: the values q 2^e, rounded to `type`.
  *   svoo_fp8_matmul: c[m][n] = act(sum_k a[m][k] b[n][k] + bias[n]) of the matrices that (a, a_scale) and (b, b_scale) stand
- *     for, accumulated in fp32 and rounded once; k counts the padded columns; b is e4m3 with a scale per row or per 128
+ *     for, rounded once; k counts the padded columns; b is e4m3 with a scale per row or per 128
  *     rows; row strides in bytes (below 2^23), rows and c at 16-byte addresses; act 0 none, 1 GELU (tanh form).  The
  *     scales of a and of b's rows may lie either way; neighbouring rows side by side are read fastest.  With 16-bit c the
- *     matrix unit cuts products 13 bits below the largest of eight before it adds them (2^-13 of the sum's size at random
- *     signs); with fp32 c the sums are fp32 throughout, at half the rate.
+ *     matrix unit cuts products 13 bits below the largest of eight before it adds them (about 2^-15 of the sum's size at
+ *     random signs) to its fp32 sums; with fp32 c the sums are fp32 throughout, at half the rate, of the operands' values as
+ *     bf16 has them (below 2^-126 in steps of 2^-133, infinite from 2^128 on).
  * ------------------------------------------------------------------------------------------- */
 int svoo_fp8_quantize_rows(const void* x, int type, long long x_row_stride, long long rows, long long cols, int fp8_type,
                            uint8_t* q, uint8_t* scale, void* stream);
