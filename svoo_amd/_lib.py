@@ -173,32 +173,46 @@ def elem_type(t: torch.Tensor, name: str) -> int:
     return _ELEM_TYPES[t.dtype]
 
 
+# What says, in a fraction of a microsecond, that nothing records tensor operations or carries tangents.  All but the first
+# are names that torch keeps to itself: without them the slower questions below are asked at every call.
+_tracing = getattr(torch._C, "_is_tracing", torch.jit.is_tracing)
+_dispatch_modes = getattr(torch._C, "_len_torch_dispatch_stack", lambda: 1)
+_function_modes = getattr(torch._C, "_len_torch_function_stack", lambda: 1)
+
+
+_forward_ad = torch.autograd.forward_ad
+
+
+def _forward_level() -> int:
+    return getattr(_forward_ad, "_current_level", 0)
+
+
 def _recorder() -> Optional[str]:
-    """What records the tensor operations of this moment, if anything does.  Some of these can only be asked of names that
-    torch keeps to itself: without them only ``torch.jit.trace`` is known."""
-    if torch.jit.is_tracing():
+    """What records the tensor operations of this moment, if anything does."""
+    if _tracing():
         return "torch.jit.trace"
-    try:
-        # both kinds of modes are on a stack while an fx graph is made; asking for that itself takes longer
-        if torch._C._len_torch_dispatch_stack() + torch._C._len_torch_function_stack() > 0 and \
-                torch.fx.experimental.proxy_tensor.get_proxy_mode() is not None:
-            return "an fx graph's tracer"
-    except AttributeError:
-        pass
+    if _dispatch_modes() or _function_modes():  # both kinds of modes are on a stack while an fx graph is made
+        try:
+            if torch.fx.experimental.proxy_tensor.get_proxy_mode() is not None:
+                return "an fx graph's tracer"
+        except AttributeError:
+            pass
     return None
 
 
 def _has_tangent(t) -> bool:
-    return isinstance(t, torch.Tensor) and torch.autograd.forward_ad.unpack_dual(t).tangent is not None
+    return isinstance(t, torch.Tensor) and _forward_ad.unpack_dual(t).tangent is not None
 
 
 def refuse_unseen(name: str, *tensors) -> None:
     """A kernel launched on raw pointers appears in no record of tensor operations, which would keep the allocation of its
     result alone, and carries no tangents: refused while such a record is made and for tensors with tangents."""
+    if not (_tracing() or _dispatch_modes() or _function_modes()) and _forward_level() < 0:
+        return
     by = _recorder()
     if by is not None:
         raise RuntimeError(f"{name} cannot be recorded by {by}")
-    if getattr(torch.autograd.forward_ad, "_current_level", 0) >= 0 and any(_has_tangent(t) for t in tensors):
+    if _forward_level() >= 0 and any(_has_tangent(t) for t in tensors):
         raise RuntimeError(f"{name} has no forward-mode derivative: call it on tensors without tangents")
 
 
@@ -208,10 +222,9 @@ def traced_or_transformed() -> bool:
     if _recorder() is not None:
         return True
     try:
-        return torch.autograd.forward_ad._current_level >= 0 or \
-            torch._C._functorch.peek_interpreter_stack() is not None
+        return _forward_level() >= 0 or torch._C._functorch.peek_interpreter_stack() is not None
     except AttributeError:
-        return False
+        return True
 
 
 def refuse_grad(name: str, *tensors) -> None:
