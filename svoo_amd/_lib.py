@@ -207,7 +207,7 @@ def _has_tangent(t) -> bool:
 def refuse_unseen(name: str, *tensors) -> None:
     """A kernel launched on raw pointers appears in no record of tensor operations, which would keep the allocation of its
     result alone, and carries no tangents: refused while such a record is made and for tensors with tangents."""
-    if not (_tracing() or _dispatch_modes() or _function_modes()) and _forward_level() < 0:
+    if not (_tracing() or _dispatch_modes() or _function_modes()) and getattr(_forward_ad, "_current_level", 0) < 0:
         return
     by = _recorder()
     if by is not None:
@@ -227,13 +227,20 @@ def traced_or_transformed() -> bool:
         return True
 
 
+def wants_grad(*tensors) -> bool:
+    """Autograd records what is made of the tensors."""
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
+
+
 def refuse_grad(name: str, *tensors) -> None:
     """An operator without a backward pass takes no tensor that waits for a gradient: its result would end the graph.
     :func:`refuse_unseen` besides."""
     refuse_unseen(name, *tensors)
-    if not torch.is_grad_enabled():
-        return
-    if any(t is not None and t.requires_grad for t in tensors):
+    if wants_grad(*tensors):
         raise RuntimeError(f"{name} has no backward pass: call it under torch.no_grad() or on detached tensors")
 
 

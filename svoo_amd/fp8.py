@@ -284,7 +284,7 @@ def fp8_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tenso
     if weight.dim() != 2 or 0 in weight.shape or x.dim() == 0 or x.shape[-1] != weight.shape[1] or \
             weight.device != x.device:
         raise ValueError(f"fp8_linear: x {tuple(x.shape)} on {x.device}, weight {tuple(weight.shape)} on {weight.device}")
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
+    if _lib.wants_grad(x, weight, bias):
         return _Linear.apply(x, weight, bias, grad_dtype)
     return _linear(x, weight, bias, False, False)[0]
 

@@ -67,16 +67,13 @@ class _Call:
             self.params, names = (scale, shift), ("scale", "shift")
         else:
             self.params, names = (weight, bias), ("weight", "bias")
-        self.keep, self.args, self.each = [], [], []
+        self.keep, self.args, self.each = keep, args, each = [], [_NO_PARAM, _NO_PARAM], [False, False]
         split = False
-        for p, name, grad in zip(self.params, names, grads):
-            args, each = _NO_PARAM, False
+        for i, p in enumerate(self.params):
             if p is not None:
-                p, args, each = _param(p, self.cols, batch, x.device, name)
-                self.keep.append(p)
-                split = split or args[2] != 0 or (each and grad)
-            self.args.append(args)
-            self.each.append(each)
+                p, args[i], each[i] = _param(p, self.cols, batch, self.device, names[i])
+                keep.append(p)
+                split = split or args[i][2] != 0 or (each[i] and grads[i])
         self.batch = batch if split else 1
         self.rows = x.numel() // self.cols // self.batch if self.batch else 0
         self.x_args = (*self.rows_of(x, x_type),)
@@ -213,7 +210,7 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
     (modulation vectors; strided ones are read in place).  Types may differ from x's.  The result has ``out_dtype``
     (x's by default).  Differentiable in x and the parameters, once."""
     _lib.refuse_unseen("layer_norm", x, weight, bias, scale, shift)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, scale, shift)):
+    if _lib.wants_grad(x, weight, bias, scale, shift):
         modulated = scale is not None or shift is not None
         if modulated and (weight is not None or bias is not None):
             raise ValueError("layer_norm: weight and bias or scale and shift, not both")
