@@ -8,7 +8,8 @@ namespace svoo {
 // with 46 of them at 1536 columns eight waves a SIMD keep enough loads in flight.  A block's rows share a batch entry,
 // whose parameters lie in LDS: in registers they would take more than the row, and loaded per row twice its bytes.
 // Measured, modulated bf16: 32760 x 1536 36 us (5.6 TB/s; 66 us with parameters and the row's values in fp32 registers),
-// 75600 x 5120 310 us (5.0 TB/s; 777 us); to 8 bits 32760 x 1536 43 us (3.5 TB/s), bound by its arithmetic as well.
+// 75600 x 5120 310 us (5.0 TB/s; 777 us); fp32 32760 x 1536 80 us (5.0 TB/s); to 8 bits 32760 x 1536 43 us (3.5 TB/s), bound
+// by its arithmetic: vector instructions fill 84 of 104 thousand cycles, of the 16-bit form 55 of 95.
 // Over other widths in whole chunks 3.7 to 5.2 TB/s (3.1 to 3.4 at 64 and 256); bf16 rows of an odd length, with no chunk
 // on a 16-byte address, 2.8 to 4.5 TB/s (to 8 bits 1.8 to 3.9): the last chunk is loaded as the row's last eight and moved
 // down (104816 x 2561 270 us; element by element, with a block per row, 587).

@@ -10,7 +10,8 @@ pytestmark = pytest.mark.gpu
 
 BF16, F16, F32 = torch.bfloat16, torch.float16, torch.float32
 
-# Every width class of the kernels (16, 64, 256 and 1024 lanes a row, one to three chunks) and both sides of its borders.
+# Every width class of the kernels (forward 16, 64 and 1024 lanes a row and one to ten chunks a lane, backward also 256 lanes
+# and one to three) and both sides of its borders.
 WIDTHS = [1, 7, 8, 24, 127, 128, 129, 511, 512, 520, 999, 1024, 1025, 1536, 1537, 2048, 2050, 4096, 4104, 5120, 6144, 6145,
           8192, 8193, 16384]
 
