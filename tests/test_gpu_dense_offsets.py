@@ -132,3 +132,39 @@ def test_linear_of_mixed_types(gpu):
         vdt, vxt = fp8_values64(d2.t().contiguous(), 1, E4)[0], fp8_values64(x2.t().contiguous(), 1, E4)[0]
         within(dw, vdt @ vxt.t(), product_bound(vdt, vxt, tw == F32))
         within(db, d2.sum(0), (m + 8) * 2.0 ** -24 * d2.abs().sum(0))
+
+
+@pytest.mark.parametrize("m,n,k", [(300, 1, 128), (65, 5, 20000), (5000, 3, 640), (70001, 1, 1100), (40000, 7, 300), (64, 2, 9000),
+                                   (100000, 130, 128), (130, 100003, 128), (256, 50000, 256)])
+def test_product_of_narrow_and_long_matrices(gpu, m, n, k):
+    """Whole numbers with a scale per row and block, so exact: one column to many, one row of tiles or one column of them."""
+    from svoo_amd import fp8
+
+    g = torch.Generator(device=gpu).manual_seed(m + n)
+    kb = -(-k // 128)
+    a, b = (torch.zeros(rows, kb * 128, device=gpu) for rows in (m, n))
+    for t in (a, b):
+        t[:, :k] = torch.randint(-2, 3, (t.shape[0], k), generator=g, device=gpu).float()
+    ea, eb = (torch.randint(-1, 2, (rows, kb), generator=g, device=gpu) for rows in (m, n))
+    sa, sb = ((e + 127).to(BYTES).t().contiguous().t().view(E8) for e in (ea, eb))
+    bias = torch.randint(-8, 9, (n,), generator=g, device=gpu).float()
+    va, vb = a.double() * spread(ea.double(), 1, *a.shape), b.double() * spread(eb.double(), 1, *b.shape)
+    want = va @ vb.t() + bias.double()
+    for out in (BF16, F32):
+        say("narrow", m, n, k, out)
+        assert torch.equal(fp8.fp8_matmul(a.to(E4), sa, b.to(E4), sb, bias, out_dtype=out), want.to(out))
+
+
+def test_operands_with_leading_dimensions_in_another_order(gpu):
+    """Values and scales whose leading dimensions are transposed, so that they are copied."""
+    from svoo_amd import fp8
+
+    g = torch.Generator(device=gpu).manual_seed(2)
+    x = torch.randn(6, 50, 300, generator=g, device=gpu).to(BF16)
+    w = fp8.fp8_quantize_blocks(torch.randn(70, 300, generator=g, device=gpu))
+    q, s = fp8.fp8_quantize_rows(x)
+    want = fp8.fp8_matmul(q, s, *w).transpose(0, 1)
+    assert torch.equal(fp8.fp8_matmul(q.transpose(0, 1), s.transpose(0, 1), *w), want)
+    assert torch.equal(fp8.fp8_dequantize(q.transpose(0, 1), s.transpose(0, 1), cols=300),
+                       fp8.fp8_dequantize(q, s, cols=300).transpose(0, 1))
+    assert torch.equal(fp8.fp8_matmul(*fp8.fp8_quantize_rows(x.transpose(0, 1)), *w), want)
