@@ -196,6 +196,10 @@ def replace_wan_linear(pipe, trainable: bool = False, grad_dtype=torch.float8_e4
         for m in part.modules():
             if _plain_linear(m):
                 _lib.elem_type(m.weight, "weight")
+                if m.bias is not None:
+                    _lib.elem_type(m.bias, "bias")
+                if 0 in m.weight.shape:
+                    raise ValueError(f"replace_wan_linear: a layer of shape {tuple(m.weight.shape)}")
     layers = []
 
     def convert(linear, activation="none"):

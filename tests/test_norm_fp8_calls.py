@@ -318,3 +318,29 @@ def test_an_ffn_with_a_forward_of_its_own_is_called(launches):
     finally:
         handle.remove()
     assert run(plain) == 1
+
+
+@pytest.mark.parametrize("trainable", [False, True])
+@pytest.mark.parametrize("spoil", ["a bias in fp64", "a weight in fp64", "a weight of nothing", "a type of gradients"])
+def test_a_pipeline_with_one_layer_that_no_call_could_take_is_left_as_it_was(launches, trainable, spoil):
+    from svoo_amd import dit
+    from svoo_amd.inference import replace_wan_linear
+
+    cfg = dit.WanDiTConfig(num_attention_heads=1, ffn_dim=64, num_layers=2, text_dim=32)
+    pipe = dit.make_pipe(cfg, dtype=torch.float32)
+    ffn = pipe.transformer.blocks[1].ffn
+    kw = {}
+    if spoil == "a bias in fp64":
+        ffn[2].bias = torch.nn.Parameter(ffn[2].bias.detach().double())
+    elif spoil == "a weight in fp64":
+        ffn[2].double()
+    elif spoil == "a weight of nothing":
+        ffn[2] = torch.nn.Linear(64, 0)
+    elif trainable:
+        kw = dict(grad_dtype=torch.bfloat16)
+    else:
+        return
+    before = {n: id(m) for n, m in pipe.transformer.named_modules()}
+    with pytest.raises((TypeError, ValueError)):
+        replace_wan_linear(pipe, trainable=trainable, **kw)
+    assert {n: id(m) for n, m in pipe.transformer.named_modules()} == before
