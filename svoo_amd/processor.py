@@ -87,11 +87,14 @@ def _apply_rotary_emb(hidden_states: torch.Tensor, freqs_cos: torch.Tensor, freq
     return out.type_as(hidden_states)
 
 
+_PROJECTIONS = ("to_q", "to_k", "to_v", "add_q_proj", "add_k_proj", "add_v_proj")
+
+
 def _refuse_lost_gradients(attn, qkv, out) -> None:
     """8-bit projections that exist to train (:class:`svoo_amd.fp8.Fp8TrainLinear`) would get no gradient through the
     sparse kernels, and no error either."""
     if torch.is_grad_enabled() and not out.requires_grad and any(t.requires_grad for t in qkv) and \
-            any(isinstance(getattr(attn, n, None), Fp8TrainLinear) for n in ("to_q", "to_k", "to_v")):
+            any(isinstance(getattr(attn, n, None), Fp8TrainLinear) for n in _PROJECTIONS):
         raise RuntimeError("sparse attention has no backward pass: trainable 8-bit projections would get no gradient "
                            "through it (run it under torch.no_grad(), or train with dense attention)")
 
@@ -738,6 +741,7 @@ class Hunyuan_SAPAttn_Processor(WanAttn_SAPAttn_Processor):
             attention_mask = torch.ones(query.shape[2], dtype=torch.bool, device=query.device)
         cu_max_seqlens = self.get_cu_max_seqlen(attention_mask, query.device)
         out = self.attention_core_logic(query, key, value, timestep, self.layer_idx, cu_max_seqlens)
+        _refuse_lost_gradients(attn, (query, key, value), out)
         out = out.transpose(1, 2).flatten(2, 3).to(query.dtype)
         return self.get_o(attn, out, encoder_hidden_states)
 

@@ -261,6 +261,30 @@ def test_attention_without_a_backward_pass_refuses_trainable_8_bit_projections(l
         assert proc(attn, x, timestep=t).shape == x.shape
 
 
+@pytest.mark.parametrize("lost", [False, True])
+def test_hunyuan_attention_refuses_trainable_8_bit_projections_too(launches, lost):
+    from types import SimpleNamespace
+
+    from svoo_amd import fp8
+    from svoo_amd.processor import Hunyuan_SAPAttn_Processor
+
+    class Processor(Hunyuan_SAPAttn_Processor):
+        def attention_core_logic(self, query, key, value, timestep, layer_idx=None, cu_max_seqlens=None):
+            out = query + key + value
+            return out.detach() if lost else out
+
+    attn = SimpleNamespace(heads=1, norm_q=None, norm_k=None, to_out=[lambda t: t] * 2,
+                           **{n: fp8.Fp8TrainLinear(64, 64) for n in ("to_q", "to_k", "to_v")})
+    proc, x, t = Processor(0), torch.randn(1, 6, 64), torch.tensor([3.0])
+    if lost:
+        with pytest.raises(RuntimeError, match="sparse attention has no backward pass"):
+            proc(attn, x, timestep=t)
+    else:
+        proc(attn, x, timestep=t)
+    with torch.no_grad():
+        proc(attn, x, timestep=t)
+
+
 # ------------------------------------------------------------------------------------------------ what no launch can hold
 def test_more_batch_entries_than_a_launch_has_blocks_are_refused():
     from svoo_amd import _lib
