@@ -278,8 +278,8 @@ int svoo_exact_sparsity_counts(const uint16_t* scores, long long rows, int n, fl
                                int32_t* counts, void* stream);
 
 /* ---------------------------------------------------------------------------------------------
- * Layer norm over rows of `cols` elements (1..16384), x [batch][rows_per_batch][cols] (fewer than 2^22 batch entries and 2^31
- * rows; pass batch 1 where nothing differs between the entries) with strides in elements and
+ * Layer norm over rows of `cols` elements (1..16384), x [batch][rows_per_batch][cols] (fewer than 2^31 rows, and than 2^24
+ * batch entries, 2^22 above 5120 columns; pass batch 1 where nothing differs between the entries) with strides in elements and
  * contiguous columns, any address.  n = (x - mean) rstd, rstd = 1 / sqrt(var + eps), statistics in fp32;
  *   y = n w + b, or with `modulated` y = n (1 + w) + b.  w and b ([cols] per batch entry, 0 as the batch stride for shared
  *   ones, NULL for none) and every other tensor have an element type: 0 bf16, 1 fp16, 2 fp32.

@@ -174,7 +174,7 @@ static unsigned grad_parts(long long batch, long long rows_per_batch, int cols) 
   return (unsigned)std::min(most, std::max(want, 1ll));
 }
 
-static int check_norm(const char* name, int x_type, long long batch, long long rows_per_batch, int cols) {
+static int check_norm(const char* name, int x_type, long long batch, long long rows_per_batch, int cols, int threads) {
   SVOO_REQUIRE(x_type >= 0 && x_type <= 2, SVOO_ERR_INVALID_ARG, "%s: element type %d (0 bf16, 1 fp16, 2 fp32)", name,
                x_type);
   SVOO_REQUIRE(batch >= 0 && rows_per_batch >= 0 && cols > 0, SVOO_ERR_INVALID_ARG,
@@ -182,8 +182,10 @@ static int check_norm(const char* name, int x_type, long long batch, long long r
   SVOO_REQUIRE(cols <= 16384, SVOO_ERR_UNSUPPORTED, "%s: %d columns (1..16384)", name, cols);
   SVOO_REQUIRE(batch < (1ll << 31) && rows_per_batch < (1ll << 31) && batch * rows_per_batch < (1ll << 31),
                SVOO_ERR_UNSUPPORTED, "%s: 2^31 rows or more", name);
-  // a block per batch entry at least: 1024 threads each have to fit a launch's 2^32
-  SVOO_REQUIRE(batch < (1ll << 22), SVOO_ERR_UNSUPPORTED, "%s: %lld batch entries (fewer than 2^22)", name, batch);
+  // a block per batch entry at least, and fewer than 2^32 threads in a launch
+  const long long most = (1ll << 32) / threads;
+  SVOO_REQUIRE(batch < most, SVOO_ERR_UNSUPPORTED, "%s: %lld batch entries of %d columns (fewer than %lld)", name, batch, cols,
+               most);
   return SVOO_OK;
 }
 
@@ -197,7 +199,7 @@ extern "C" int svoo_layer_norm_fwd(const void* x, int x_type, long long x_batch_
                                    long long rows_per_batch, int cols, void* y, int y_type, uint8_t* q, uint8_t* q_scale,
                                    int fp8_type, float* mean, float* rstd, void* stream) {
   static const char* name = "svoo_layer_norm_fwd";
-  if (const int rc = check_norm(name, x_type, batch, rows_per_batch, cols)) return rc;
+  if (const int rc = check_norm(name, x_type, batch, rows_per_batch, cols, cols <= 5120 ? 256 : 1024)) return rc;
   SVOO_REQUIRE(w_type >= 0 && w_type <= 2 && b_type >= 0 && b_type <= 2 && y_type >= 0 && y_type <= 2,
                SVOO_ERR_INVALID_ARG, "%s: element types %d %d %d (0 bf16, 1 fp16, 2 fp32)", name, w_type, b_type, y_type);
   SVOO_REQUIRE(fp8_type == kFp8E4m3 || fp8_type == kFp8E5m2, SVOO_ERR_INVALID_ARG, "%s: 8-bit type %d (0 e4m3, 1 e5m2)",
@@ -247,7 +249,7 @@ extern "C" int svoo_layer_norm_bwd(const void* x, int x_type, long long x_batch_
                                    void* dw, int dw_type, void* db, int db_type, void* workspace, size_t ws_bytes,
                                    void* stream) {
   static const char* name = "svoo_layer_norm_bwd";
-  if (const int rc = check_norm(name, x_type, batch, rows_per_batch, cols)) return rc;
+  if (const int rc = check_norm(name, x_type, batch, rows_per_batch, cols, cols <= 6144 ? 256 : 1024)) return rc;
   SVOO_REQUIRE(dy_type >= 0 && dy_type <= 2 && w_type >= 0 && w_type <= 2 && dw_type >= 0 && dw_type <= 2 &&
                    db_type >= 0 && db_type <= 2,
                SVOO_ERR_INVALID_ARG, "%s: element types %d %d %d %d (0 bf16, 1 fp16, 2 fp32)", name, dy_type, w_type,

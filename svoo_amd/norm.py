@@ -3,7 +3,7 @@
 A DiT block norms its hidden states three times and modulates two of them (``svoo/models/wan/custom_models.py:23-109``);
 as tensor operations that is five to seven passes over the activations, here one read and one write.  Statistics are
 fp32 whatever the tensors' types (bf16, fp16, fp32), outputs are rounded once.  Rows of 1 to 16384 columns, any strides
-between rows and batch entries; fewer than 2^22 batch entries where a parameter has a row for each.
+between rows and batch entries; fewer than 2^24 batch entries (2^22 above 5120 columns) where a parameter has a row for each.
 
 :func:`layer_norm` is differentiable.  :func:`layer_norm_fwd` and :func:`layer_norm_bwd` are its two passes as plain
 calls, for programs that keep the statistics themselves or capture a training step into a graph (autograd ties a leaf's

@@ -139,3 +139,22 @@ def test_shared_gradients_in_a_graph(gpu, batch, rows, cols):
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(out, want[i % 2])), i
         assert all(torch.equal(a, b) for a, b in zip(step(*data[1]), want[1]))
+
+
+@pytest.mark.parametrize("batch,cols", [((1 << 22) + 5, 9), ((1 << 24) - 1, 8)])
+def test_parameters_of_millions_of_batch_entries(gpu, batch, cols):
+    """A row and a parameter each: as in calls of the ends alone."""
+    from svoo_amd import norm
+
+    g = torch.Generator(device=gpu).manual_seed(cols)
+    x, dy = (torch.randn(batch, cols, generator=g, device=gpu).to(BF16) for _ in range(2))
+    sc, sh = (torch.randn(batch, cols, generator=g, device=gpu) for _ in range(2))
+    say("millions of entries", batch, cols)
+    y, mean, rstd = norm.layer_norm_fwd(x, scale=sc, shift=sh)
+    grads = norm.layer_norm_bwd(dy, x, mean, rstd, scale=sc, shift=sh)
+    for at in (slice(0, 100), slice(batch // 2, batch // 2 + 100), slice(batch - 100, batch)):
+        y1, mean1, rstd1 = norm.layer_norm_fwd(x[at], scale=sc[at], shift=sh[at])
+        assert torch.equal(y[at], y1) and torch.equal(mean[at], mean1) and torch.equal(rstd[at], rstd1)
+        ends = norm.layer_norm_bwd(dy[at], x[at], mean1, rstd1, scale=sc[at], shift=sh[at])
+        assert all(torch.equal(a[at], b) for a, b in zip(grads, ends))
+    assert torch.equal(grads[2], dy.float())  # one row an entry

@@ -290,13 +290,13 @@ def test_more_batch_entries_than_a_launch_has_blocks_are_refused():
     from svoo_amd import _lib
 
     lib = _lib.lib()
-    for batch in (1 << 22, 1 << 30):
-        assert lib.svoo_layer_norm_fwd(16, 0, 8, 8, 16, 2, 8, None, 2, 0, 1, 1e-6, batch, 1, 8, 16, 0, None, None, 0, None,
-                                       None, None) == -2
-        assert f"{batch} batch entries" in _lib.last_error()
-        assert lib.svoo_layer_norm_bwd(16, 0, 8, 8, 16, 0, 8, 8, None, 2, 0, 1, 16, 16, batch, 1, 8, 16, 16, 2, 16, 2, None, 0,
-                                       None) == -2
-        assert f"{batch} batch entries" in _lib.last_error()
+    for batch, cols in ((1 << 24, 8), (1 << 30, 8), (1 << 24, 5120), (1 << 22, 6145), (1 << 22, 16384)):
+        assert lib.svoo_layer_norm_fwd(16, 0, cols, cols, 16, 2, cols, None, 2, 0, 1, 1e-6, batch, 1, cols, 16, 0, None, None,
+                                       0, None, None, None) == -2
+        assert f"{batch} batch entries of {cols} columns" in _lib.last_error()
+        assert lib.svoo_layer_norm_bwd(16, 0, cols, cols, 16, 0, cols, cols, None, 2, 0, 1, 16, 16, batch, 1, cols, 16, 16, 2,
+                                       16, 2, None, 0, None) == -2
+        assert f"{batch} batch entries of {cols} columns" in _lib.last_error()
 
 
 # ------------------------------------------------------------------------------------------------ an FFN that is someone else's
