@@ -337,6 +337,79 @@ int svoo_fp8_matmul(const uint8_t* a, long long a_row_stride, const uint8_t* a_s
                     void* c, int c_type, void* workspace, size_t ws_bytes, void* stream);
 
 /* ---------------------------------------------------------------------------------------------
+ * A gated residual and the layer norm behind it (beside svoo/models/wan/custom_models.py:23-109): x, b, dh and dy are
+ * [batch][rows][cols] by strides in elements with contiguous columns, all of one element type (0 bf16, 1 fp16, 2 fp32);
+ * parameters as svoo_layer_norm_fwd's, the gate too (NULL: 1); 1..16384 columns, batch below 65536.
+ *   svoo_residual_norm_fwd: h = x + gate b in the type, and of h as stored y = n w + c (`modulated`: n (1 + w) + c); without y
+ *     the residual alone.  h and y are contiguous; mean and rstd (fp32, one per row) are optional.
+ *   svoo_residual_norm_bwd: for gradients dh and dy (either may be NULL) of h and y: dx, db (contiguous, the type), and the sums
+ *     dgate, dw, dc, each optional, with a row per batch entry where *_per_batch says so, else over all rows.  The sums are
+ *     fp32 in a fixed order and need the workspace.
+ * ------------------------------------------------------------------------------------------- */
+int svoo_residual_norm_fwd(const void* x, int type, long long x_batch_stride, long long x_row_stride, const void* b,
+                           long long b_batch_stride, long long b_row_stride, const void* gate, int gate_type,
+                           long long gate_batch_stride, const void* w, int w_type, long long w_batch_stride, const void* c,
+                           int c_type, long long c_batch_stride, int modulated, float eps, long long batch, long long rows,
+                           int cols, void* h, void* y, float* mean, float* rstd, void* stream);
+size_t svoo_residual_norm_bwd_workspace_size(long long batch, long long rows, int cols);
+int svoo_residual_norm_bwd(const void* dh, long long dh_batch_stride, long long dh_row_stride, const void* dy,
+                           long long dy_batch_stride, long long dy_row_stride, int type, const void* h, const void* b,
+                           long long b_batch_stride, long long b_row_stride, const void* gate, int gate_type,
+                           long long gate_batch_stride, const void* w, int w_type, long long w_batch_stride, int modulated,
+                           const float* mean, const float* rstd, long long batch, long long rows, int cols, void* dx, void* db,
+                           void* dgate, int dgate_type, int dgate_per_batch, void* dw, int dw_type, int dw_per_batch, void* dc,
+                           int dc_type, int dc_per_batch, void* workspace, size_t ws_bytes, void* stream);
+
+/* ---------------------------------------------------------------------------------------------
+ * Rotary positions on several axes behind an RMS norm (svoo/models/wan/attention.py:153-190): x [batch][rows][heads][d] by
+ * strides in elements with contiguous columns, d even, up to 512.  norm: 0 none, 1 over a token's heads (at most
+ * 32 floor(64 / ceil(d / 8)) of them), 2 per head; w [heads * d] or [d] or NULL.  Pair j of an axis of c channels turns by
+ * p theta^(-2j / c) (1 to 4 axes; host arrays); pairs are neighbours, or with `halves` channel j of a head's two halves.
+ * pos_type: 0 positions of a grid (host array of sizes, the last axis fastest, counted from grid_start or 0; rows behind it
+ * are not turned), 1 int32, 2 int64, 3 fp32 positions [batch][rows][axes] with pos_batch_stride elements between entries.
+ *   svoo_axis_rope_fwd: y contiguous, x's type.
+ *   svoo_axis_rope_bwd: dx (contiguous, x's type) and dw for the incoming dy, each optional; dw needs the workspace and is
+ *     an fp32 sum in a fixed order.  x may be NULL without a norm.
+ * ------------------------------------------------------------------------------------------- */
+int svoo_axis_rope_fwd(const void* x, int type, long long x_batch_stride, long long x_row_stride, long long x_head_stride,
+                       long long batch, long long rows, int heads, int d, int norm, const void* w, int w_type, float eps,
+                       int axes, const int* axis_channels, const double* theta, const int* grid, const int* grid_start,
+                       const void* positions, int pos_type, long long pos_batch_stride, int halves, void* y, void* stream);
+size_t svoo_axis_rope_bwd_workspace_size(long long batch, long long rows, int heads, int d, int norm);
+int svoo_axis_rope_bwd(const void* dy, long long dy_batch_stride, long long dy_row_stride, long long dy_head_stride,
+                       const void* x, int type, long long x_batch_stride, long long x_row_stride, long long x_head_stride,
+                       long long batch, long long rows, int heads, int d, int norm, const void* w, int w_type, float eps,
+                       int axes, const int* axis_channels, const double* theta, const int* grid, const int* grid_start,
+                       const void* positions, int pos_type, long long pos_batch_stride, int halves, void* dx, void* dw,
+                       int dw_type, void* workspace, size_t ws_bytes, void* stream);
+
+/* ---------------------------------------------------------------------------------------------
+ * Dense attention with a backward pass (no reference counterpart: the reference calls the framework's).  q [batch][heads][sq][d],
+ * k and v [batch][kv_heads][sk][d] by strides in elements, columns contiguous, rows at 16-byte addresses (strides in multiples
+ * of 8); type 0 bf16, 1 fp16; d a multiple of 8 up to 128; heads a multiple of kv_heads; scale above 0.  q_lens and k_lens
+ * (device int32 [batch] or NULL, clamped to 0..sq and 0..sk): rows behind them are not read and have o = 0 and no gradient.
+ *   svoo_dense_attention_fwd: o [batch][sq][heads][d] contiguous, o_rest (optional) what its rounding left, in the same type
+ *     and layout, for a backward pass of full accuracy, and lse [batch][heads][sq] (fp32, -inf for queries without keys).
+ *   svoo_dense_attention_bwd: dq [batch][sq][heads][d], dk and dv [batch][sk][kv_heads][d], contiguous, each optional; the same
+ *     call gives the same bits.  The workspace lies at a 16-byte address.
+ * ------------------------------------------------------------------------------------------- */
+size_t svoo_dense_attention_fwd_workspace_size(int batch, int heads, int sq, int sk, int d);
+int svoo_dense_attention_fwd(const void* q, long long q_batch, long long q_head, long long q_row, const void* k,
+                             long long k_batch, long long k_head, long long k_row, const void* v, long long v_batch,
+                             long long v_head, long long v_row, int type, int batch, int heads, int kv_heads, int sq, int sk,
+                             int d, float scale, const int32_t* q_lens, const int32_t* k_lens, void* o, void* o_rest,
+                             float* lse, void* workspace, size_t ws_bytes, void* stream);
+size_t svoo_dense_attention_bwd_workspace_size(int type, int batch, int heads, int kv_heads, int sq, int sk, int d, int want_q,
+                                               int want_kv);
+int svoo_dense_attention_bwd(const void* dy, long long dy_batch, long long dy_head, long long dy_row, const void* q,
+                             long long q_batch, long long q_head, long long q_row, const void* k, long long k_batch,
+                             long long k_head, long long k_row, const void* v, long long v_batch, long long v_head,
+                             long long v_row, const void* o, long long o_batch, long long o_head, long long o_row,
+                             const void* o_rest, const float* lse, int type, int batch, int heads, int kv_heads, int sq, int sk, int d,
+                             float scale, const int32_t* q_lens, const int32_t* k_lens, void* dq, void* dk, void* dv,
+                             void* workspace, size_t ws_bytes, void* stream);
+
+/* ---------------------------------------------------------------------------------------------
  * Diagnostic (no reference counterpart): runs one v_mfma_f32_32x32x16_bf16 and one
  * v_mfma_f32_16x16x32_bf16 on index-coded operands and writes the raw per-lane accumulators
  * (out32: 64 lanes x 16 floats, out16: 64 lanes x 4 floats), so tests can confirm the operand

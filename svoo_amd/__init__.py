@@ -16,6 +16,7 @@ from .co_clustering import (  # noqa: F401
     triton_l2norm_forward,
     weighted_softmax,
 )
+from .dense import dense_attention, dense_attention_bwd, dense_attention_fwd  # noqa: F401
 from .fp8 import (  # noqa: F401
     Fp8Linear,
     Fp8TrainLinear,
@@ -26,7 +27,16 @@ from .fp8 import (  # noqa: F401
     fp8_quantize_both,
     fp8_quantize_rows,
 )
-from .norm import layer_norm, layer_norm_bwd, layer_norm_fp8, layer_norm_fwd  # noqa: F401
+from .norm import (  # noqa: F401
+    gated_residual,
+    layer_norm,
+    layer_norm_bwd,
+    layer_norm_fp8,
+    layer_norm_fwd,
+    residual_norm,
+    residual_norm_bwd,
+    residual_norm_fwd,
+)
 from .permute import (  # noqa: F401
     apply_inverse_permutation,
     apply_inverse_permutation_triton,
@@ -34,6 +44,7 @@ from .permute import (  # noqa: F401
     permute_tensor_by_labels,
     permute_tensor_by_labels_triton,
 )
+from .rope import axis_rope, axis_rope_bwd  # noqa: F401
 from .sparsity import SparsityLookup  # noqa: F401
 
 __version__ = "0.1.0"

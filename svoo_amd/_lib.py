@@ -71,6 +71,26 @@ _SIGS = {
     "svoo_fp8_matmul_workspace_size": (c_size_t, [c_longlong, c_longlong, c_longlong, c_int]),
     "svoo_fp8_matmul": (c_int, [P, c_longlong, P, c_longlong, c_longlong, c_int, P, c_longlong, P, c_longlong, c_longlong,
                                 c_int, P, c_int, c_int, c_longlong, c_longlong, c_longlong, P, c_int, P, c_size_t, P]),
+    "svoo_residual_norm_fwd": (c_int, [P, c_int, c_longlong, c_longlong, P, c_longlong, c_longlong, P, c_int, c_longlong,
+                                       P, c_int, c_longlong, P, c_int, c_longlong, c_int, c_float, c_longlong, c_longlong,
+                                       c_int, P, P, P, P, P]),
+    "svoo_residual_norm_bwd_workspace_size": (c_size_t, [c_longlong, c_longlong, c_int]),
+    "svoo_residual_norm_bwd": (c_int, [P, c_longlong, c_longlong, P, c_longlong, c_longlong, c_int, P, P, c_longlong,
+                                       c_longlong, P, c_int, c_longlong, P, c_int, c_longlong, c_int, P, P, c_longlong,
+                                       c_longlong, c_int, P, P, P, c_int, c_int, P, c_int, c_int, P, c_int, c_int, P,
+                                       c_size_t, P]),
+    "svoo_axis_rope_fwd": (c_int, [P, c_int, c_longlong, c_longlong, c_longlong, c_longlong, c_longlong, c_int, c_int, c_int,
+                                   P, c_int, c_float, c_int, P, P, P, P, P, c_int, c_longlong, c_int, P, P]),
+    "svoo_axis_rope_bwd_workspace_size": (c_size_t, [c_longlong, c_longlong, c_int, c_int, c_int]),
+    "svoo_axis_rope_bwd": (c_int, [P, c_longlong, c_longlong, c_longlong, P, c_int, c_longlong, c_longlong, c_longlong,
+                                   c_longlong, c_longlong, c_int, c_int, c_int, P, c_int, c_float, c_int, P, P, P, P, P,
+                                   c_int, c_longlong, c_int, P, P, c_int, P, c_size_t, P]),
+    "svoo_dense_attention_fwd_workspace_size": (c_size_t, [c_int, c_int, c_int, c_int, c_int]),
+    "svoo_dense_attention_fwd": (c_int, [P, c_longlong, c_longlong, c_longlong] * 3 + [c_int] * 7 +
+                                 [c_float, P, P, P, P, P, P, c_size_t, P]),
+    "svoo_dense_attention_bwd_workspace_size": (c_size_t, [c_int] * 9),
+    "svoo_dense_attention_bwd": (c_int, [P, c_longlong, c_longlong, c_longlong] * 5 + [P, P] + [c_int] * 7 +
+                                 [c_float, P, P, P, P, P, P, c_size_t, P]),
     "svoo_vbsa_ear_fwd": (c_int, [P, P, P, P, P, P, P, P, P, c_int, c_int, c_int, c_int, c_int, P, c_size_t, P, P]),
 }
 

@@ -228,3 +228,178 @@ def layer_norm_fp8(x, weight=None, bias=None, *, scale=None, shift=None, eps=1e-
     q, s = empty_fp8(x.shape[:-1], c.cols, dtype, x.device), empty_scales(x.shape[:-1], c.cols, x.device)
     c.forward(None, c.x_args[1], q.data_ptr(), s.data_ptr(), FP8_TYPES[dtype], None, None)
     return q, s
+
+
+# ------------------------------------------------------------------------------------------------ gated residuals
+class _Residual:
+    """The checked arguments of a gated residual with or without a norm: tensors as ``[batch, rows, cols]``, the parameters
+    ``(gate, weight or scale, bias or shift)``.  Rows are split by batch entries where a parameter's values differ between
+    them or a gradient with a row per entry is wanted (``grads``, of the three parameters)."""
+
+    __slots__ = ("x", "kind", "cols", "eps", "device", "shape", "batch", "rows", "modulated", "params", "args", "each", "keep")
+
+    def __init__(self, name, x, gate, weight, bias, scale, shift, eps, grads=(False,) * 3):
+        self.modulated = scale is not None or shift is not None
+        if self.modulated and (weight is not None or bias is not None):
+            raise ValueError(f"{name}: weight and bias or scale and shift, not both")
+        if not eps >= 0:
+            raise ValueError(f"{name}: eps={eps}")
+        self.kind = _lib.elem_type(x, "x")
+        self.shape = shape = x.shape
+        if len(shape) == 0 or not 1 <= shape[-1] <= 16384:
+            raise ValueError(f"{name}: x of shape {tuple(shape)} (1..16384 columns)")
+        self.x, self.cols, self.eps, self.device = x, shape[-1], eps, x.device
+        batch = shape[0] if len(shape) > 1 else 1
+        self.params = (gate, scale, shift) if self.modulated else (gate, weight, bias)
+        names = ("gate", "scale", "shift") if self.modulated else ("gate", "weight", "bias")
+        self.keep, self.args, self.each = [], [_NO_PARAM] * 3, [False] * 3
+        split = False
+        for i, p in enumerate(self.params):
+            if p is not None:
+                p, self.args[i], self.each[i] = _param(p, self.cols, batch, self.device, names[i])
+                self.keep.append(p)
+                split = split or self.args[i][2] != 0 or (self.each[i] and grads[i])
+        self.batch = batch if split else 1
+        if self.batch >= 65536:
+            raise ValueError(f"{name}: {self.batch} batch entries with parameters of their own (fewer than 65536)")
+        self.rows = x.numel() // self.cols // self.batch if self.batch else 0
+
+    def rows_of(self, t, name):
+        """A tensor of x's shape and type as the C entries take it, ``(pointer, batch stride, row stride)``."""
+        if _lib.elem_type(t, name) != self.kind or t.shape != self.shape or t.device != self.device:
+            raise ValueError(f"{name}: {t.dtype} {tuple(t.shape)} on {t.device}, x {self.x.dtype} {tuple(self.shape)} on "
+                             f"{self.device}")
+        if t.is_contiguous():
+            return t.data_ptr(), self.rows * self.cols, self.cols
+        t = t.reshape(self.batch, self.rows, self.cols)
+        if t.stride(2) != 1 and self.cols > 1:
+            t = t.contiguous()
+        self.keep.append(t)
+        return t.data_ptr(), t.stride(0), t.stride(1)
+
+
+def _residual_forward(c: _Residual, branch, normed: bool, stats: bool):
+    """``(h, y or None, statistics [2, rows] or None)``."""
+    at, *strides = c.rows_of(c.x, "x")
+    b_args = c.rows_of(branch, "branch")
+    h = torch.empty(c.shape, dtype=c.x.dtype, device=c.device)
+    y = torch.empty(c.shape, dtype=c.x.dtype, device=c.device) if normed else None
+    rows = c.batch * c.rows
+    st = torch.empty((2, rows), dtype=torch.float32, device=c.device) if stats else None
+    mean = st.data_ptr() if stats else None
+    _lib.launch(c.device, "svoo_residual_norm_fwd", at, c.kind, *strides, *b_args, *c.args[0], *c.args[1], *c.args[2],
+                c.modulated, c.eps, c.batch, c.rows, c.cols, h.data_ptr(), _lib.ptr(y), mean, mean + 4 * rows if stats else None)
+    return h, y, st
+
+
+def _residual_backward(c: _Residual, dh, dy, h, branch, mean, rstd, needs):
+    """``(dx, dbranch, dgate, dweight, dbias)`` as ``needs`` says; dy, h and the statistics are None for a residual alone."""
+    params = c.params
+    want = [p is not None and bool(n) for p, n in zip(params, needs[2:])]
+    new = [torch.empty(c.shape, dtype=c.x.dtype, device=c.device) if n else None for n in needs[:2]]
+    if c.batch * c.rows == 0:
+        return (*new, *(torch.zeros_like(p) if w else None for p, w in zip(params, want)))
+    sums = [torch.empty(p.shape, dtype=p.dtype, device=c.device) if w else None for p, w in zip(params, want)]
+    if not any(needs[:2]) and not any(want):
+        return (*new, *sums)
+    size, ws = 0, None
+    if any(want):
+        size = _lib.lib().svoo_residual_norm_bwd_workspace_size(c.batch, c.rows, c.cols)
+        ws = _lib.workspace(size, c.device)
+    none = (None, 0, 0)
+    _lib.launch(c.device, "svoo_residual_norm_bwd", *(none if dh is None else c.rows_of(dh, "dh")),
+                *(none if dy is None else c.rows_of(dy, "dy")), c.kind, _lib.ptr(h),
+                *(c.rows_of(branch, "branch") if want[0] else none), *c.args[0], *c.args[1], c.modulated, mean, rstd, c.batch,
+                c.rows, c.cols, *(_lib.ptr(t) for t in new),
+                *(v for i, t in enumerate(sums) for v in (_lib.ptr(t), 2 if t is None else _lib.elem_type(t, ""), c.each[i])),
+                _lib.ptr(ws), size)
+    return (*new, *sums)
+
+
+class _ResidualNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, branch, gate, p0, p1, modulated, eps):
+        norm = (None, None, p0, p1) if modulated else (p0, p1, None, None)
+        h, y, st = _residual_forward(_Residual("residual_norm", x, gate, *norm, eps), branch, True, True)
+        ctx.save_for_backward(h, branch if gate is not None and gate.requires_grad else None, gate, p0, p1, st)
+        ctx.modulated, ctx.eps = modulated, eps
+        return h, y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dh, dy):
+        h, branch, gate, p0, p1, st = ctx.saved_tensors
+        needs = ctx.needs_input_grad[:5]
+        norm = (None, None, p0, p1) if ctx.modulated else (p0, p1, None, None)
+        c = _Residual("residual_norm", h, gate, *norm, ctx.eps, needs[2:])
+        at = st.data_ptr()
+        return (*_residual_backward(c, dh, dy, h, branch, at, at + 4 * st.shape[1], needs), None, None)
+
+
+class _GatedResidual(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, branch, gate):
+        c = _Residual("gated_residual", x, gate, None, None, None, None, 0.0)
+        h = _residual_forward(c, branch, False, False)[0]
+        ctx.save_for_backward(branch if gate is not None and gate.requires_grad else None, gate)
+        return h
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dh):
+        branch, gate = ctx.saved_tensors
+        need_x, need_b, need_g = ctx.needs_input_grad
+        dx = dh if need_x else None
+        if gate is None:
+            return dx, dh if need_b else None, None
+        c = _Residual("gated_residual", dh, gate, None, None, None, None, 0.0, (need_g, False, False))
+        _, db, dg, _, _ = _residual_backward(c, dh, None, None, branch, None, None, (False, need_b, need_g, False, False))
+        return dx, db, dg
+
+
+def residual_norm(x: torch.Tensor, branch: torch.Tensor, gate: Optional[torch.Tensor] = None,
+                  weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None, *,
+                  scale: Optional[torch.Tensor] = None, shift: Optional[torch.Tensor] = None, eps: float = 1e-6):
+    """``(h, y)``: ``h = x + gate * branch``, rounded to x's type, and :func:`layer_norm` of h in the same pass.
+
+    ``branch`` has x's shape and type; ``gate`` (1 without one) and the norm's parameters are as those of
+    :func:`layer_norm`.  Differentiable in all of them, once."""
+    _lib.refuse_unseen("residual_norm", x, branch, gate, weight, bias, scale, shift)
+    if _lib.wants_grad(x, branch, gate, weight, bias, scale, shift):
+        modulated = scale is not None or shift is not None
+        if modulated and (weight is not None or bias is not None):
+            raise ValueError("residual_norm: weight and bias or scale and shift, not both")
+        return _ResidualNorm.apply(x, branch, gate, scale if modulated else weight, shift if modulated else bias, modulated,
+                                   eps)
+    c = _Residual("residual_norm", x, gate, weight, bias, scale, shift, eps)
+    return _residual_forward(c, branch, True, False)[:2]
+
+
+def gated_residual(x: torch.Tensor, branch: torch.Tensor, gate: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``x + gate * branch``, rounded once to x's type, without a norm: a block's end.  Differentiable, once."""
+    _lib.refuse_unseen("gated_residual", x, branch, gate)
+    if _lib.wants_grad(x, branch, gate):
+        return _GatedResidual.apply(x, branch, gate)
+    return _residual_forward(_Residual("gated_residual", x, gate, None, None, None, None, 0.0), branch, False, False)[0]
+
+
+def residual_norm_fwd(x, branch, gate=None, weight=None, bias=None, *, scale=None, shift=None, eps=1e-6):
+    """``(h, y, mean, rstd)`` of :func:`residual_norm`, with the fp32 statistics of every row of h.  No autograd."""
+    _lib.refuse_grad("residual_norm_fwd", x, branch, gate, weight, bias, scale, shift)
+    c = _Residual("residual_norm_fwd", x, gate, weight, bias, scale, shift, eps)
+    h, y, st = _residual_forward(c, branch, True, True)
+    return h, y, st[0].view(x.shape[:-1]), st[1].view(x.shape[:-1])
+
+
+def residual_norm_bwd(dh, dy, h, branch, mean, rstd, gate=None, weight=None, bias=None, *, scale=None, shift=None, eps=1e-6,
+                      needs: Sequence[bool] = (True,) * 5):
+    """Gradients ``(dx, dbranch, dgate, dweight, dbias)`` (dscale and dshift in the last two places) for the gradients that
+    arrive at h (or None) and y, from what :func:`residual_norm_fwd` took and returned; None without a parameter or where
+    ``needs`` says so.  Sums over rows are fp32 in a fixed order."""
+    _lib.refuse_unseen("residual_norm_bwd", dh, dy, h, branch, mean, rstd, gate, weight, bias, scale, shift)
+    for t, name in ((mean, "mean"), (rstd, "rstd")):
+        if not isinstance(t, torch.Tensor) or t.dtype != torch.float32 or t.shape != h.shape[:-1] or t.device != h.device:
+            raise ValueError(f"{name}: fp32 of shape {tuple(h.shape[:-1])} on {h.device} expected")
+    mean, rstd = mean.contiguous(), rstd.contiguous()
+    c = _Residual("residual_norm_bwd", h, gate, weight, bias, scale, shift, eps, needs[2:])
+    return _residual_backward(c, dh, dy, h.contiguous(), branch, mean.data_ptr(), rstd.data_ptr(), needs)
