@@ -145,7 +145,9 @@ dense_fwd_kernel(DenseArgs a) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) mx = fmaxf(mx, sacc[kb2][r]);
       mx = xhalf_max(mx) * sl;
-      const float m_new = fmaxf(m_run, mx);
+      // a row's maximum moves for its own sake alone: its bits do not depend on the rows beside it
+      const bool moves = xhalf_max(lsum <= 8192.0f ? 0.0f : 1.0f) > 0.0f;
+      const float m_new = moves ? fmaxf(m_run, mx) : m_run;
       const float alpha = __builtin_amdgcn_exp2f(m_run - m_new);
       m_run = m_new;
       l_run *= alpha;
