@@ -119,9 +119,12 @@ class WanBlock(nn.Module):
 
     With ``fused_norms`` each norm and its modulation are one pass (:func:`svoo_amd.norm.layer_norm`, differentiable) in
     place of the norm modules' calls (which stay where the block is traced, transformed or under forward-mode AD), and an
-    8-bit FFN (:func:`svoo_amd.inference.replace_wan_linear`) takes its input as 8-bit rows from the norm."""
+    8-bit FFN (:func:`svoo_amd.inference.replace_wan_linear`) takes its input as 8-bit rows from the norm.  With
+    ``fused_residuals`` besides, a branch, its gate and the stream join in the pass of the norm that follows
+    (:func:`svoo_amd.norm.residual_norm`), h rounded once where the tensor operations round a product and a sum."""
 
     fused_norms = False
+    fused_residuals = False
 
     def __init__(self, cfg: WanDiTConfig):
         super().__init__()
@@ -145,25 +148,49 @@ class WanBlock(nn.Module):
         else:
             x = (self.norm1(hidden_states.float()) * (1 + scale) + shift).to(dtype)
         a = self.attn1(hidden_states=x, rotary_emb=rotary_emb, timestep=timestep)
+        if fused and self.fused_residuals:
+            return self._residuals(hidden_states, a, encoder_hidden_states, mod)
         hidden_states = (hidden_states.float() + a.float() * gate).to(dtype)
         if fused:
             x = norm.layer_norm(hidden_states, self.norm2.weight, self.norm2.bias, eps=self.norm2.eps)
         else:
             x = self.norm2(hidden_states.float()).to(dtype)
         hidden_states = hidden_states + self.attn2(hidden_states=x, encoder_hidden_states=encoder_hidden_states)
-        if fused and type(self.ffn) is nn.Sequential and type(self.ffn[0]) is Fp8Linear and \
-                not _watched(self.ffn, self.ffn[0]):
-            rows = norm.layer_norm_fp8(hidden_states, scale=c_scale, shift=c_shift, eps=self.norm3.eps)
-            first, *rest = self.ffn
-            f = first.forward_quantized(*rows, out_dtype=dtype)
-            for layer in rest:
-                f = layer(f)
+        if fused and self._quantized_ffn():
+            f = self._ffn_of_rows(hidden_states, c_scale, c_shift)
         elif fused:
             f = self.ffn(norm.layer_norm(hidden_states, scale=c_scale, shift=c_shift, eps=self.norm3.eps))
         else:
             x = (self.norm3(hidden_states.float()) * (1 + c_scale) + c_shift).to(dtype)
             f = self.ffn(x)
         return (hidden_states.float() + f.float() * c_gate).to(dtype)
+
+    def _quantized_ffn(self) -> bool:
+        return type(self.ffn) is nn.Sequential and type(self.ffn[0]) is Fp8Linear and not _watched(self.ffn, self.ffn[0])
+
+    def _ffn_of_rows(self, hidden_states, scale, shift):
+        """An 8-bit FFN from the norm's 8-bit rows."""
+        rows = norm.layer_norm_fp8(hidden_states, scale=scale, shift=shift, eps=self.norm3.eps)
+        first, *rest = self.ffn
+        f = first.forward_quantized(*rows, out_dtype=hidden_states.dtype)
+        for layer in rest:
+            f = layer(f)
+        return f
+
+    def _residuals(self, hidden_states, a, encoder_hidden_states, mod):
+        """The block behind self-attention, each residual in the pass of the norm behind it."""
+        _, _, gate, c_shift, c_scale, c_gate = mod
+        dtype = hidden_states.dtype
+        hidden_states, x = norm.residual_norm(hidden_states, a.to(dtype), gate, self.norm2.weight, self.norm2.bias,
+                                              eps=self.norm2.eps)
+        a = self.attn2(hidden_states=x, encoder_hidden_states=encoder_hidden_states).to(dtype)
+        if self._quantized_ffn():
+            hidden_states = norm.gated_residual(hidden_states, a)
+            f = self._ffn_of_rows(hidden_states, c_scale, c_shift)
+        else:
+            hidden_states, x = norm.residual_norm(hidden_states, a, scale=c_scale, shift=c_shift, eps=self.norm3.eps)
+            f = self.ffn(x)
+        return norm.gated_residual(hidden_states, f.to(dtype), c_gate)
 
 
 def timestep_embedding(t: torch.Tensor, dim: int) -> torch.Tensor:
@@ -214,10 +241,13 @@ class WanDiT(nn.Module):
         self._rope = None
         self.fused_norms = False
 
-    def fuse_norms(self, on: bool = True) -> "WanDiT":
-        """Norms and modulations of every block and of the head as single passes on the GPU (off by default)."""
+    def fuse_norms(self, on: bool = True, residuals: bool = False) -> "WanDiT":
+        """Norms and modulations of every block and of the head as single passes on the GPU (off by default); with
+        ``residuals`` the blocks' gated residuals join the passes of the norms behind them."""
         for m in (self, *self.blocks):
             m.fused_norms = on
+        for m in self.blocks:
+            m.fused_residuals = on and residuals
         return self
 
     def rope(self, f: int, h: int, w: int, device):

@@ -13,7 +13,7 @@ the same for HunyuanVideo 1.0 (``svoo/models/hunyuan10/inference.py:31-231``): o
 :class:`Hunyuan_SAPAttn_Processor` per double-stream block (layers ``0 .. D-1``), then per
 single-stream block (layers ``D ..``), the numbering the per-layer profile CSV is indexed by.
 
-``replace_wan_linear`` puts 8-bit linear layers into the blocks of a Wan pipeline; it has no counterpart in the reference.
+``replace_wan_attention_trainable`` installs dense attention with gradients, and ``replace_wan_linear`` puts 8-bit linear layers into the blocks of a Wan pipeline; neither has a counterpart in the reference.
 """
 
 from __future__ import annotations
@@ -25,7 +25,7 @@ import torch
 from . import _lib
 from .fp8 import Fp8Linear, Fp8TrainLinear
 from .processor import (Hunyuan_SAPAttn_Processor, WanAttn_DenseAttn_Processor, WanAttn_EARAttn_Processor,
-                        WanAttn_SAPAttn_Processor)
+                        WanAttn_SAPAttn_Processor, WanAttn_TrainAttn_Processor)
 from .sparsity import SparsityLookup
 from .sparsity.exact import resume_requested
 
@@ -161,6 +161,30 @@ def replace_wan_attention(
                 proc.num_layers = num_layers
                 block.attn1.set_processor(proc)
                 processors.append(proc)
+    return processors
+
+
+def replace_wan_attention_trainable(pipe, height: int, width: int, num_frames: int, theta: float = 10000.0):
+    """Install dense attention with gradients (:class:`svoo_amd.processor.WanAttn_TrainAttn_Processor`) in ``attn1`` and
+    ``attn2`` of every block of a Wan pipeline's transformers, for training on clips of this size.
+
+    The transformer is bf16 or fp16, with head dims up to 128 and no image branch (``ValueError`` before the first change).
+    ``theta`` is the rotary base, 10000 for every Wan model.  Returns the processors."""
+    patch = pipe.transformer.config.patch_size
+    frames, _ = wan_token_geometry(pipe, height, width, num_frames)
+    mod_h, mod_w = (pipe.vae_scale_factor_spatial * p for p in patch[1:])
+    d = pipe.transformer.config.attention_head_dim
+    if not 1 <= d <= 128 or d % 2:
+        raise ValueError(f"replace_wan_attention_trainable: head dim {d}")
+    blocks = [b for t in (pipe.transformer, getattr(pipe, "transformer_2", None)) if t is not None for b in t.blocks]
+    layers = [a for b in blocks for a in (b.attn1, getattr(b, "attn2", None)) if a is not None]
+    if any(getattr(a, "add_k_proj", None) is not None for a in layers):
+        raise ValueError("replace_wan_attention_trainable: an image branch")
+    hw = 2 * (d // 6)
+    processors = []
+    for a in layers:
+        a.set_processor(WanAttn_TrainAttn_Processor((frames, height // mod_h, width // mod_w), (d - 2 * hw, hw, hw), theta))
+        processors.append(a.processor)
     return processors
 
 

@@ -15,12 +15,15 @@ configuration of ``svoo/models/wan/attention.py:546-1216``:
 pruning error) and the attention for its centroid-compensated form
 (``svoo/models/wan/attention.py:1047-1071, 1180-1196, 1219-1222``).
 
+``WanAttn_TrainAttn_Processor`` (no reference counterpart) is dense attention on kernels with a backward pass, for training.
+
 ``Hunyuan_SAPAttn_Processor`` adds the text-dense post-processing of
 ``svoo/models/hunyuan10/attention.py:977-1110`` on the same kernels.
 """
 
 from __future__ import annotations
 
+import math
 import os
 from typing import Optional
 
@@ -33,7 +36,7 @@ from .ear import dynamic_block_sparse_prune_fwd, ear_map_and_value_centroids
 from .sparsity.exact import (compute_exact_attention_sparsity, format_sparsity_log, has_completed_sparsity_entry,
                              record_sparsity_entry)
 from .permute import apply_inverse_permutation, apply_inverse_permutation_bshd, permute_pair_by_indices
-from . import _lib, heads
+from . import _lib, dense, heads, rope
 from .fp8 import Fp8TrainLinear
 
 
@@ -583,6 +586,65 @@ class WanAttn_DenseAttn_Processor(WanAttn_SAPAttn_Processor):
             f"Query Shape: {seq_len} is not equivalent to {self.context_length} + {self.num_frame} * {self.frame_size}"
         )
         return self.flash_attention(query, key, value).transpose(1, 2).flatten(2, 3)
+
+
+class WanAttn_TrainAttn_Processor:
+    """Dense self- and cross-attention of a Wan block on kernels with gradients: q/k norm and rotary positions in one pass
+    (:func:`svoo_amd.rope.axis_rope`), attention and its backward pass by :func:`svoo_amd.dense.dense_attention`.
+
+    ``grid`` is the clip's latent frames, rows and columns; positions are the grid's, and the tables that a block passes as
+    ``rotary_emb`` only say that there is a rotation.  bf16 or fp16, no attention mask, no image branch.  Where operators are
+    traced or transformed, or tensors have tangents, tensor operations compute the same."""
+
+    def __init__(self, grid, axes, theta: float = 10000.0):
+        self.grid, self.axes, self.theta = tuple(grid), tuple(axes), theta
+
+    def _heads(self, norm, x, heads: int, rotated: bool):
+        width = x.shape[-1]
+        weight, eps, over = None, 0.0, "none"
+        if norm is not None:
+            if type(norm) is getattr(torch.nn, "RMSNorm", None) and norm.normalized_shape == (width,) and \
+                    norm.eps is not None and not heads_module_watched(norm):
+                weight, eps, over = norm.weight, norm.eps, "row"
+            else:
+                x = norm(x)
+        x = x.unflatten(2, (heads, -1))
+        if rotated:
+            return rope.axis_rope(x, self.axes, grid=self.grid, theta=self.theta, norm=over, weight=weight, eps=eps)
+        return x if over == "none" else rope.axis_rope(x, (0,), grid=(1,), norm=over, weight=weight, eps=eps)
+
+    def __call__(self, attn, hidden_states, encoder_hidden_states=None, attention_mask=None, rotary_emb=None, timestep=None):
+        if attention_mask is not None or getattr(attn, "add_k_proj", None) is not None:
+            raise ValueError("WanAttn_TrainAttn_Processor: no attention mask and no image branch")
+        if rotary_emb is not None and hidden_states.shape[1] != math.prod(self.grid):
+            raise ValueError(f"WanAttn_TrainAttn_Processor: {hidden_states.shape[1]} tokens for a grid of {self.grid}")
+        context = hidden_states if encoder_hidden_states is None else encoder_hidden_states
+        if encoder_hidden_states is None and getattr(attn, "fused_projections", False):
+            q, k, v = attn.to_qkv(hidden_states).chunk(3, dim=-1)
+        else:
+            q, k, v = attn.to_q(hidden_states), attn.to_k(context), attn.to_v(context)
+        norms = getattr(attn, "norm_q", None), getattr(attn, "norm_k", None)
+        if _lib.traced_or_transformed():
+            q, k = (t if n is None else n(t) for n, t in zip(norms, (q, k)))
+            q, k, v = (t.unflatten(2, (attn.heads, -1)) for t in (q, k, v))
+            if rotary_emb is not None:
+                q, k = _apply_rotary_emb(q, *rotary_emb), _apply_rotary_emb(k, *rotary_emb)
+            q, k, v = (t.transpose(1, 2) for t in (q, k, v))
+            if _lib._forward_level() >= 0:  # torch's fused attention has no forward-mode derivative
+                scores = q @ k.transpose(2, 3).contiguous() * q.shape[-1] ** -0.5
+                o = torch.softmax(scores, -1) @ v.contiguous()
+            else:
+                o = F.scaled_dot_product_attention(q, k, v)
+        else:
+            q, k = (self._heads(n, t, attn.heads, rotary_emb is not None) for n, t in zip(norms, (q, k)))
+            o = dense.dense_attention(*(t.transpose(1, 2) for t in (q, k, v.unflatten(2, (attn.heads, -1)))))
+        return attn.to_out[1](attn.to_out[0](o.transpose(1, 2).flatten(2)))
+
+
+def heads_module_watched(m) -> bool:
+    """Something waits for a call of the module: hooks, its own or every module's, or a forward set on it."""
+    return "forward" in m.__dict__ or any(getattr(torch.nn.modules.module, n, None) for n in heads.GLOBAL_HOOKS) or \
+        any(getattr(m, n) for n in heads.MODULE_HOOKS)
 
 
 def _apply_rotary_emb_real(x: torch.Tensor, freqs_cis) -> torch.Tensor:
