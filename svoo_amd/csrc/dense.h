@@ -99,20 +99,24 @@ __device__ __forceinline__ int seq_len(const int32_t* lens, int b, int most) {
 }
 
 // Rows row0 .. of a matrix into an LDS tile of kRows x DP by LDS DMA, issued by kWaves waves (this one the w-th); rows behind
-// `last` repeat it.  A scalar base and 32-bit offsets: 64 rows are below 2^31 bytes apart.  Columns from d on are left as
+// `last` repeat it.  A scalar base and 32-bit offsets: rows are below 2^24 bytes apart.  Columns from d on are left as
 // they are (tile_clear).
 template <int DP, bool kFull, int kRows, int kWaves>
 __device__ __forceinline__ void tile_dma(const uint16_t* base, long long row_stride, int row0, int last, int d, uint16_t* tile,
                                          int w, int lane) {
-  constexpr int kChunks = DP / 8, kIt = kRows * kChunks / (64 * kWaves);
+  constexpr int kChunks = DP / 8, kIt = kRows * kChunks / (64 * kWaves), kEach = 64 / kChunks;  // rows of a copy
+  w = __builtin_amdgcn_readfirstlane(w);
   const int first = min(row0, last), most = last - first;
   const char* from = (const char*)(base + first * row_stride);
   const uint32_t step = (uint32_t)row_stride * 2;
-  __asm__ volatile("" : "+v"(lane));  // places made here: kept from tile to tile they take registers that the sums need
+  uint32_t l = lane;
+  __asm__ volatile("" : "+v"(l));  // places made here: kept from tile to tile they take registers that the sums need
+  // row n kEach + l / kChunks has chunk l % kChunks where the swizzle of the lane's part of the row and of n's put it
+  const uint32_t row = l / kChunks, chunk = l % kChunks ^ (DP == 128 ? row << 2 : l / 16);
 #pragma unroll
   for (int j = 0; j < kIt; ++j) {
-    const int p = (w * kIt + j) * 64 + lane, r = p / kChunks, c = tile_swz<DP>(r, p % kChunks);
-    if (kFull || c * 8 < d) lds_dma16(from + ((uint32_t)min(r, most) * step + (uint32_t)c * 16), tile + (w * kIt + j) * 64 * 8);
+    const uint32_t n = w * kIt + j, c = chunk ^ (DP == 128 ? n & 3 : (n & 1) << 2);
+    if (kFull || c * 8 < (uint32_t)d) lds_dma16(from + (__umul24(min(n * kEach + row, (uint32_t)most), step) + c * 16), tile + n * 64 * 8);
   }
 }
 // Tiles with columns that no copy fills, once: zeros.
@@ -163,25 +167,38 @@ __device__ __forceinline__ unsigned xcd_block(unsigned bid, unsigned total) {
 
 // Four values to 16 bits, and what that leaves of them.
 template <int T>
-__device__ __forceinline__ void store4(uint16_t* to, uint16_t* rest, f32x4_t v) {
-  const uint2 w = make_uint2(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]));
-  *(uint2*)to = w;
-  if (rest != nullptr)
-    *(uint2*)rest = make_uint2(pack2<T>(v[0] - elem16<T>(w.x, 0), v[1] - elem16<T>(w.x, 1)),
-                               pack2<T>(v[2] - elem16<T>(w.y, 0), v[3] - elem16<T>(w.y, 1)));
+__device__ __forceinline__ uint2 pack4(f32x4_t v) { return make_uint2(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3])); }
+template <int T>
+__device__ __forceinline__ f32x4_t rest4(f32x4_t v, uint2 w) {
+  return f32x4_t{v[0] - elem16<T>(w.x, 0), v[1] - elem16<T>(w.x, 1), v[2] - elem16<T>(w.y, 0), v[3] - elem16<T>(w.y, 1)};
 }
-// acc [columns][row of this lane] to a contiguous row of 16-bit elements or fp32.
+// Two groups of eight columns, of which each lane of a pair (l, l + 32) holds four: the first group whole in the lower lane,
+// the second in the upper one.
+__device__ __forceinline__ u32x4_t join_halves(uint2 a, uint2 b) {
+  const auto x = __builtin_amdgcn_permlane32_swap(a.x, b.x, false, false), y = __builtin_amdgcn_permlane32_swap(a.y, b.y, false, false);
+  return u32x4_t{x[0], y[0], x[1], y[1]};
+}
+// acc [columns][row of this lane] to a contiguous row of 16-bit elements, both lanes of a row together.
 template <int T, int DP, bool kFull>
 __device__ __forceinline__ void store_row16(uint16_t* row, uint16_t* rest, const f32x16_t (&acc)[DP / 32], int d, int h,
                                             float by) {
 #pragma unroll
   for (int db = 0; db < DP / 32; ++db)
 #pragma unroll
-    for (int r4 = 0; r4 < 4; ++r4) {
-      const int c = 32 * db + 8 * r4 + 4 * h;
-      if (kFull || c < d)
-        store4<T>(row + c, rest != nullptr ? rest + c : nullptr,
-                  f32x4_t{acc[db][4 * r4], acc[db][4 * r4 + 1], acc[db][4 * r4 + 2], acc[db][4 * r4 + 3]} * by);
+    for (int pair = 0; pair < 2; ++pair) {
+      const int c = 32 * db + 16 * pair + 8 * h;
+      f32x4_t v[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[i][e] = acc[db][8 * pair + 4 * i + e] * by;
+      const uint2 a = pack4<T>(v[0]), b = pack4<T>(v[1]);
+      const u32x4_t w = join_halves(a, b);
+      if (kFull || c < d) *(u32x4_t*)(row + c) = w;
+      if (rest != nullptr) {
+        const u32x4_t r = join_halves(pack4<T>(rest4<T>(v[0], a)), pack4<T>(rest4<T>(v[1], b)));
+        if (kFull || c < d) *(u32x4_t*)(rest + c) = r;
+      }
     }
 }
 template <int DP, bool kFull>

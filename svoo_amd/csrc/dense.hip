@@ -241,7 +241,10 @@ __global__ void __launch_bounds__(256) dense_join_kernel(DenseArgs a) {
   const float by = l > 0.0f || l != l ? 1.0f / lw : 0.0f;
   const int row = (int)(at % a.sq), bh = (int)(at / a.sq);
   const size_t to = ((size_t)(bh / a.heads) * a.sq + row) * a.heads * a.d + (size_t)(bh % a.heads) * a.d + c;
-  store4<T>(a.out + to, a.rest != nullptr ? a.rest + to : nullptr, o * by);
+  o *= by;
+  const uint2 w = pack4<T>(o);
+  *(uint2*)(a.out + to) = w;
+  if (a.rest != nullptr) *(uint2*)(a.rest + to) = pack4<T>(rest4<T>(o, w));
   if (c == 0) a.lse[at] = l > 0.0f || l != l ? (m + __builtin_amdgcn_logf(l)) * kLn2 : -INFINITY;
 }
 
@@ -265,7 +268,7 @@ static int fwd_splits(int batch, int heads, int sq, int sk, int d) {
 }
 
 bool dense_rows_ok(const DenseRows& m) {
-  return (uintptr_t)m.p % 16 == 0 && m.batch % 8 == 0 && m.head % 8 == 0 && m.row % 8 == 0 && m.row >= 0 && m.row < (1 << 24);
+  return (uintptr_t)m.p % 16 == 0 && m.batch % 8 == 0 && m.head % 8 == 0 && m.row % 8 == 0 && m.row >= 0 && m.row < (1 << 23);
 }
 int check_dense(const char* name, int type, int batch, int heads, int kv_heads, int sq, int sk, int d) {
   SVOO_REQUIRE(type == kDenseBf16 || type == kDenseF16, SVOO_ERR_INVALID_ARG, "%s: element type %d (0 bf16, 1 fp16)", name, type);

@@ -85,6 +85,13 @@ __device__ __forceinline__ float f16_exponent(const DenseArgs& a, int b, int kv,
 // next, so that matrix and vector units are busy at the same time: without the two groups, waves of a block that meet at
 // every tile's barrier do the same thing at the same time, and a step takes the sum of both (dq 8.8 ms at 12 x 32760 x 128).
 // A step is 32 rows of the other side, half a tile; group B copies tile t + 1 during step 2 t, into the buffer of tile t - 1.
+// Matrix work goes first where both want to issue (7.4 ms and 7.2 of dq at full clocks, 8.5 and 8.4 at the power limit).
+template <class Matrix>
+__device__ __forceinline__ void raised(Matrix matrix, int u) {
+  __builtin_amdgcn_s_setprio(1);
+  matrix(u);
+  __builtin_amdgcn_s_setprio(0);
+}
 template <class Scores, class Matrix, class Vector, class Copy, class Wait>
 __device__ __forceinline__ void alternate(int tiles, bool group_b, bool active, Scores scores, Matrix matrix, Vector vector,
                                           Copy copy, Wait wait) {
@@ -99,7 +106,7 @@ __device__ __forceinline__ void alternate(int tiles, bool group_b, bool active, 
   const int n = 2 * tiles;
   for (int u = 0; u < n; ++u) {
     if (!group_b) {
-      if (active) matrix(u);
+      if (active) raised(matrix, u);
     } else {
       if (u % 2 == 0 && u + 2 < n) copy(u / 2 + 1);
       if (active) vector(u);
@@ -108,7 +115,7 @@ __device__ __forceinline__ void alternate(int tiles, bool group_b, bool active, 
     if (!group_b) {
       if (active && u + 1 < n) vector(u + 1);
     } else {
-      if (active) matrix(u);
+      if (active) raised(matrix, u);
       if (u % 2 == 0 && u + 2 < n) wait(u / 2 + 1);
     }
     __syncthreads();
@@ -120,7 +127,7 @@ __device__ __forceinline__ void alternate(int tiles, bool group_b, bool active, 
 template <int T, int DP, bool kFull>
 __global__ void __launch_bounds__(kBwdWaves * kWave) __attribute__((amdgpu_waves_per_eu(2, 2)))
 dense_dq_kernel(DenseArgs a) {
-  constexpr int kS = DP / 16, kB = DP / 32, kElems = kBwdTile * DP;
+  constexpr int kAhead = 2, kS = DP / 16, kB = DP / 32, kElems = kBwdTile * DP;
   __shared__ __attribute__((aligned(16))) uint16_t k_s[2 * kElems], v_s[2 * kElems];
   __shared__ float scratch[2 * kBwdWaves];
   const unsigned total = (unsigned)a.batch * a.heads * a.tiles * a.splits, item = xcd_block(blockIdx.x, total);
@@ -167,31 +174,31 @@ dense_dq_kernel(DenseArgs a) {
     // operands are read two instructions ahead
     auto products = [&](auto sums, const uint16_t* kt, const uint16_t* kn, const uint16_t* vn) __attribute__((always_inline)) {
       constexpr int kSums = decltype(sums)::value ? 2 * kB : 0, kAll = kSums + 2 * kS;
-      u32x4_t op[3];
+      u32x4_t op[kAhead + 1];
       auto operand = [&](int i) __attribute__((always_inline)) -> u32x4_t {
         if (i < kSums) return at.cols(kt + i / kB * 16 * DP, i % kB);
         return at.row((i - kSums) % 2 ? vn : kn, (i - kSums) / 2);
       };
-      op[0] = operand(0);
-      op[1] = operand(1);
-      if (kSums) __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
-      else __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) op[i] = operand(i);
+      if (kSums) __builtin_amdgcn_sched_group_barrier(0x100, 2 * kAhead, 0);
+      else __builtin_amdgcn_sched_group_barrier(0x100, kAhead, 0);
 #pragma unroll
       for (int i = 0; i < kAll; ++i) {
-        if (i + 2 < kAll) {
-          op[(i + 2) % 3] = operand(i + 2);
-          if (i + 2 < kSums) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+        if (i + kAhead < kAll) {
+          op[(i + kAhead) % (kAhead + 1)] = operand(i + kAhead);
+          if (i + kAhead < kSums) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
           else __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
         }
         const int n = i - kSums;
         if (i < kSums) {
-          acc[i % kB] = mma<T>(op[i % 3], ds[i / kB], acc[i % kB]);
+          acc[i % kB] = mma<T>(op[i % (kAhead + 1)], ds[i / kB], acc[i % kB]);
         } else if (n % 2 == 0) {
           if (n == 0) s = f32x16_t{};
-          s = mma<T>(op[i % 3], qop[n / 2], s);
+          s = mma<T>(op[i % (kAhead + 1)], qop[n / 2], s);
         } else {
           if (n == 1) dp = f32x16_t{};
-          dp = mma<T>(op[i % 3], dop[n / 2], dp);
+          dp = mma<T>(op[i % (kAhead + 1)], dop[n / 2], dp);
         }
         __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
       }
@@ -237,7 +244,7 @@ dense_dq_kernel(DenseArgs a) {
 template <int T, int DP, bool kFull>
 __global__ void __launch_bounds__(kBwdWaves * kWave) __attribute__((amdgpu_waves_per_eu(2, 2)))
 dense_dkv_kernel(DenseArgs a) {
-  constexpr int kS = DP / 16, kB = DP / 32, kElems = kBwdTile * DP;
+  constexpr int kAhead = 2, kS = DP / 16, kB = DP / 32, kElems = kBwdTile * DP;
   __shared__ __attribute__((aligned(16))) uint16_t q_s[2 * kElems], d_s[2 * kElems], v_s[kBwdRows * DP];
   __shared__ __attribute__((aligned(16))) float stat_s[2][2][kBwdTile];  // -L log2(e) (fp16: + 14), -D
   __shared__ float scratch[2 * kBwdWaves];
@@ -301,36 +308,36 @@ dense_dkv_kernel(DenseArgs a) {
     auto products = [&](auto sums, const uint16_t* qt_s, const uint16_t* dt_s, const uint16_t* qn, const uint16_t* dn)
                         __attribute__((always_inline)) {
       constexpr int kSums = decltype(sums)::value ? 4 * kB : 0, kAll = kSums + 2 * kS;
-      u32x4_t op[3], vop[2];
+      u32x4_t op[kAhead + 1], vop[kAhead / 2 + 1];
       at.forget();
       auto operand = [&](int i) __attribute__((always_inline)) -> u32x4_t {
         if (i < kSums) return at.cols((i % 2 ? qt_s : dt_s) + i / 2 / kB * 16 * DP, i / 2 % kB);
         const int n = i - kSums;
-        if (n % 2) vop[n / 2 % 2] = at.row(vt, n / 2);
+        if (n % 2) vop[n / 2 % (kAhead / 2 + 1)] = at.row(vt, n / 2);
         return at.row(n % 2 ? dn : qn, n / 2);
       };
-      op[0] = operand(0);
-      op[1] = operand(1);
-      if (kSums) __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
-      else __builtin_amdgcn_sched_group_barrier(0x100, 3, 0);
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) op[i] = operand(i);
+      if (kSums) __builtin_amdgcn_sched_group_barrier(0x100, 2 * kAhead, 0);
+      else __builtin_amdgcn_sched_group_barrier(0x100, kAhead + kAhead / 2, 0);
 #pragma unroll
       for (int i = 0; i < kAll; ++i) {
         const int n = i - kSums;
-        if (i + 2 < kAll) {
-          op[(i + 2) % 3] = operand(i + 2);
-          if (i + 2 < kSums || (i + 2 - kSums) % 2) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+        if (i + kAhead < kAll) {
+          op[(i + kAhead) % (kAhead + 1)] = operand(i + kAhead);
+          if (i + kAhead < kSums || (i + kAhead - kSums) % 2) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
           else __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
         }
         if (i < kSums) {
           const int db = i / 2 % kB, st = i / 2 / kB;
-          if (i % 2) dk[db] = mma<T>(op[i % 3], ds[st], dk[db]);
-          else dv[db] = mma<T>(op[i % 3], p[st], dv[db]);
+          if (i % 2) dk[db] = mma<T>(op[i % (kAhead + 1)], ds[st], dk[db]);
+          else dv[db] = mma<T>(op[i % (kAhead + 1)], p[st], dv[db]);
         } else if (n % 2 == 0) {
           if (n == 0) s = f32x16_t{};
-          s = mma<T>(op[i % 3], kop[n / 2], s);
+          s = mma<T>(op[i % (kAhead + 1)], kop[n / 2], s);
         } else {
           if (n == 1) dp = f32x16_t{};
-          dp = mma<T>(op[i % 3], vop[n / 2 % 2], dp);
+          dp = mma<T>(op[i % (kAhead + 1)], vop[n / 2 % (kAhead / 2 + 1)], dp);
         }
         __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
       }

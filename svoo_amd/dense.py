@@ -77,7 +77,7 @@ class _Call:
         if self.dp != self.d:
             t = torch.nn.functional.pad(t, (0, self.dp - self.d))
         st = [s if n > 1 else 0 for s, n in zip(t.stride(), t.shape)]
-        if (st[3] != 1 and self.dp > 1) or t.data_ptr() % 16 or st[0] % 8 or st[1] % 8 or st[2] % 8:
+        if (st[3] != 1 and self.dp > 1) or t.data_ptr() % 16 or st[0] % 8 or st[1] % 8 or st[2] % 8 or st[2] >= 1 << 23:
             t = t.contiguous()
             st = t.stride()
             if t.data_ptr() % 16:  # contiguous as it was, at another address

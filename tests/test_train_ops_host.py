@@ -39,7 +39,7 @@ SHARED = [
     (dict(sq=(1 << 30) + 1), -2, "up to 2^30"), (dict(sk=1 << 30, batch=2), -2, "tiles of 256"), (dict(scale=0.0), -1, "scale=0"),
     (dict(scale=-1.0), -1, "scale=-1"), (dict(scale=math.inf), -1, "scale=inf"), (dict(scale=math.nan), -1, "scale=nan"),
     (dict(q=None), -1, "null pointer"), (dict(k=None), -1, "null pointer"), (dict(lse=None), -1, "null pointer"),
-    (dict(q=8), -1, "16-byte"), (dict(k_r=130), -1, "16-byte"), (dict(v_h=4), -1, "16-byte"), (dict(q_r=1 << 24), -1, "16-byte"),
+    (dict(q=8), -1, "16-byte"), (dict(k_r=130), -1, "16-byte"), (dict(v_h=4), -1, "16-byte"), (dict(q_r=1 << 23), -1, "16-byte"),
     (dict(q_r=-128), -1, "16-byte"),
 ]
 
