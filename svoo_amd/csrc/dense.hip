@@ -219,33 +219,58 @@ dense_fwd_kernel(DenseArgs a) {
   }
 }
 
-// Joins the shares of a query's keys: a thread takes four columns.
+// Joins the shares of a query's keys.  A thread takes four columns and every eighth share, and the eight meet in LDS: a query
+// over a long cache has a hundred shares (one thread after another 16 us, this 5).
+constexpr int kJoinSlices = 8;
 template <int T>
 __global__ void __launch_bounds__(256) dense_join_kernel(DenseArgs a) {
-  const int per_row = a.d / 4;
-  const size_t rows = (size_t)a.batch * a.heads * a.sq, i = (size_t)blockIdx.x * 256 + threadIdx.x, at = i / per_row;
-  if (at >= rows) return;
-  const int c = (int)(i % per_row) * 4;
-  float m = -INFINITY;
-  for (int s = 0; s < a.splits; ++s) m = fmaxf(m, a.part_ml[s * rows + at].x);
+  __shared__ f32x4_t s_o[256];
+  __shared__ float s_m[256], s_l[256], s_w[256];
+  const int per_row = a.d / 4, here = 256 / (per_row * kJoinSlices);  // rows of a block
+  const int c = threadIdx.x % per_row, slice = threadIdx.x / per_row % kJoinSlices, mine = threadIdx.x / (per_row * kJoinSlices);
+  const size_t rows = (size_t)a.batch * a.heads * a.sq, at = (size_t)blockIdx.x * here + mine;
+  const bool on = mine < here && at < rows;
+  float m = -INFINITY, l = 0.0f, lw = 0.0f;
   f32x4_t o = {0, 0, 0, 0};
-  float l = 0.0f, lw = 0.0f;
-  for (int s = 0; s < a.splits; ++s) {
-    const float4 ml = a.part_ml[s * rows + at];
-    if (ml.x == -INFINITY && !(ml.y != ml.y)) continue;  // an empty share wrote no row
-    const float w = __builtin_amdgcn_exp2f(ml.x - m);
-    l = fmaf(ml.y, w, l);
-    lw = fmaf(ml.z, w, lw);
-    o += *(const f32x4_t*)(a.part + (s * rows + at) * a.d + c) * w;
+  if (on) {
+    for (int s = slice; s < a.splits; s += kJoinSlices) m = fmaxf(m, a.part_ml[s * rows + at].x);
+#pragma unroll 4
+    for (int s = slice; s < a.splits; s += kJoinSlices) {
+      const float4 ml = a.part_ml[s * rows + at];
+      if (ml.x == -INFINITY && !(ml.y != ml.y)) continue;  // an empty share wrote no row
+      const float w = __builtin_amdgcn_exp2f(ml.x - m);
+      l = fmaf(ml.y, w, l);
+      lw = fmaf(ml.z, w, lw);
+      o += *(const f32x4_t*)(a.part + (s * rows + at) * a.d + 4 * c) * w;
+    }
   }
-  const float by = l > 0.0f || l != l ? 1.0f / lw : 0.0f;
+  s_o[threadIdx.x] = o;
+  s_m[threadIdx.x] = m;
+  s_l[threadIdx.x] = l;
+  s_w[threadIdx.x] = lw;
+  __syncthreads();
+  if (!on || slice != 0) return;
+#pragma unroll
+  for (int i = 1; i < kJoinSlices; ++i) m = fmaxf(m, s_m[threadIdx.x + i * per_row]);
+  o = f32x4_t{0, 0, 0, 0};
+  l = lw = 0.0f;
+#pragma unroll
+  for (int i = 0; i < kJoinSlices; ++i) {
+    const int j = threadIdx.x + i * per_row;
+    if (s_m[j] == -INFINITY && !(s_l[j] != s_l[j])) continue;
+    const float w = __builtin_amdgcn_exp2f(s_m[j] - m);
+    l = fmaf(s_l[j], w, l);
+    lw = fmaf(s_w[j], w, lw);
+    o += s_o[j] * w;
+  }
+  const bool some = l > 0.0f || l != l;
   const int row = (int)(at % a.sq), bh = (int)(at / a.sq);
-  const size_t to = ((size_t)(bh / a.heads) * a.sq + row) * a.heads * a.d + (size_t)(bh % a.heads) * a.d + c;
-  o *= by;
+  const size_t to = ((size_t)(bh / a.heads) * a.sq + row) * a.heads * a.d + (size_t)(bh % a.heads) * a.d + 4 * c;
+  o *= some ? 1.0f / lw : 0.0f;
   const uint2 w = pack4<T>(o);
   *(uint2*)(a.out + to) = w;
   if (a.rest != nullptr) *(uint2*)(a.rest + to) = pack4<T>(rest4<T>(o, w));
-  if (c == 0) a.lse[at] = l > 0.0f || l != l ? (m + __builtin_amdgcn_logf(l)) * kLn2 : -INFINITY;
+  if (c == 0) a.lse[at] = some ? (m + __builtin_amdgcn_logf(l)) * kLn2 : -INFINITY;
 }
 
 // Shares of the contracted length for a launch of `blocks` blocks that each walk over `units` tiles: the fewest rounds of 256
@@ -335,11 +360,12 @@ extern "C" int svoo_dense_attention_fwd(const void* q, long long q_batch, long l
   a.part_ml = (float4*)((float*)workspace + (need ? (size_t)a.splits * rows * d : 0));
   const unsigned total = (unsigned)batch * heads * a.tiles * a.splits;
   const dim3 grid((total + 7) / 8 * 8), block(kFwdWaves * kWave);
+  const size_t joined = 256 / (d / 4 * kJoinSlices);  // rows of a joining block
   for_dense(type, d, [&](auto t, auto dp, auto full) {
     constexpr int kT = decltype(t)::value;
     hipLaunchKernelGGL((dense_fwd_kernel<kT, decltype(dp)::value, decltype(full)::value>), grid, block, 0, (hipStream_t)stream, a);
     if (a.splits > 1)
-      hipLaunchKernelGGL((dense_join_kernel<kT>), dim3((unsigned)((rows * (d / 4) + 255) / 256)), dim3(256), 0,
+      hipLaunchKernelGGL((dense_join_kernel<kT>), dim3((unsigned)((rows + joined - 1) / joined)), dim3(256), 0,
                          (hipStream_t)stream, a);
   });
   return check_launch(name);
