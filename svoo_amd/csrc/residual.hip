@@ -320,7 +320,7 @@ static int row_groups(int cols) { return cols <= 128 ? 16 : cols <= 1536 ? 4 : 1
 // Blocks that share a batch entry's rows in the backward pass, whose partial sums are joined at the end.
 static unsigned residual_parts(long long batch, long long rows, int cols) {
   const long long groups = row_groups(cols);
-  const long long most = std::max(1024 / batch, 1ll), want = (rows + 4 * groups - 1) / (4 * groups);
+  const long long most = std::max(512 / batch, 1ll), want = (rows + 4 * groups - 1) / (4 * groups);
   return (unsigned)std::min(most, std::max(want, 1ll));
 }
 
@@ -374,7 +374,7 @@ extern "C" int svoo_residual_norm_fwd(const void* x, int type, long long x_batch
   for_residual_width(cols, [&](auto tpr, auto nc) {
     constexpr int kTpr = decltype(tpr)::value, kNc = decltype(nc)::value, kThreads = kTpr > 256 ? kTpr : 256;
     const long long groups = kThreads / kTpr, want = (rows + groups - 1) / groups;
-    a.parts = (unsigned)std::min(want, std::max(256 * (2048 / kThreads) / batch, 1ll));
+    a.parts = (unsigned)std::min(want, std::max(std::max(512 / (kThreads / 256), 256) / batch, 1ll));
     for_residual_type(type, [&](auto t) {
       for_residual_flag(cols % 8 == 0, [&](auto whole) {
         hipLaunchKernelGGL((residual_fwd_kernel<decltype(t)::value, kTpr, kNc, decltype(whole)::value>),

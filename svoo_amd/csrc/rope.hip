@@ -432,7 +432,7 @@ static unsigned rope_blocks(long long tokens, int heads, int d, int norm, bool g
   const int lanes = (d + 7) / 8, hpw = kWave / lanes;
   if (norm == kNormRow) {
     const long long groups = heads <= 3 * hpw || (!grad && heads <= 10 * hpw) ? 4 : 1;
-    return (unsigned)std::min<long long>((tokens + groups - 1) / groups, grad ? 512 : 2048);
+    return (unsigned)std::min<long long>((tokens + groups - 1) / groups, grad ? 512 : 1024);
   }
   *head_step = (unsigned)std::min(heads, 16);
   *head_blocks = (unsigned)((heads + *head_step - 1) / *head_step);

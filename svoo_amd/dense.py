@@ -52,8 +52,7 @@ class _Call:
         self.kind = _kind(q, "q")
         self.dtype, self.device = q.dtype, q.device
         for t, name in ((k, "k"), (v, "v")):
-            _kind(t, name)
-            if t.dtype != q.dtype or t.device != q.device:
+            if _kind(t, name) != self.kind or t.device != self.device:
                 raise ValueError(f"{name}: {t.dtype} on {t.device}, q {q.dtype} on {q.device}")
         if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape or q.shape[0] != k.shape[0] or q.shape[3] != k.shape[3]:
             raise ValueError(f"dense_attention: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}; [B, H, S, D], "
@@ -74,20 +73,26 @@ class _Call:
     def rows(self, t):
         """``(pointer, elements between batch entries, heads and rows)`` of an operand, copied where it cannot be read in
         place."""
-        if self.dp != self.d:
+        if self.dp == self.d:
+            at, (b, h, r, c) = t.data_ptr(), t.stride()
+            if c == 1 and not (at | 2 * (b | h | r)) % 16 and r < 1 << 23:
+                return at, b, h, r
+        else:
             t = torch.nn.functional.pad(t, (0, self.dp - self.d))
-        st = [s if n > 1 else 0 for s, n in zip(t.stride(), t.shape)]
-        if (st[3] != 1 and self.dp > 1) or t.data_ptr() % 16 or st[0] % 8 or st[1] % 8 or st[2] % 8 or st[2] >= 1 << 23:
+        b, h, r, c = (s if n > 1 else 0 for s, n in zip(t.stride(), t.shape))  # strides of single entries do not count
+        if (c != 1 and self.dp > 1) or (t.data_ptr() | 2 * (b | h | r)) % 16 or r >= 1 << 23:
             t = t.contiguous()
-            st = t.stride()
             if t.data_ptr() % 16:  # contiguous as it was, at another address
                 t = t.clone()
+            b, h, r, _ = t.stride()
         self.keep.append(t)
-        return t.data_ptr(), st[0], st[1], st[2]
+        return t.data_ptr(), b, h, r
 
     def empty(self, heads: int, rows: int):
         """A result ``[B, H, S, D]``, contiguous as ``[B, S, H, D]``: a block's ``transpose(1, 2).flatten(2)`` is free."""
-        return torch.empty(self.batch, rows, heads, self.dp, dtype=self.dtype, device=self.device).transpose(1, 2)
+        d = self.dp
+        return torch.empty_strided((self.batch, heads, rows, d), (rows * heads * d, d, heads * d, 1), dtype=self.dtype,
+                                   device=self.device)
 
     def cut(self, t):
         if t is None or self.dp == self.d:
