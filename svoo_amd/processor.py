@@ -604,7 +604,7 @@ class WanAttn_TrainAttn_Processor:
         weight, eps, over = None, 0.0, "none"
         if norm is not None:
             if type(norm) is getattr(torch.nn, "RMSNorm", None) and norm.normalized_shape == (width,) and \
-                    norm.eps is not None and not heads_module_watched(norm):
+                    norm.eps is not None and not _module_watched(norm):
                 weight, eps, over = norm.weight, norm.eps, "row"
             else:
                 x = norm(x)
@@ -641,7 +641,7 @@ class WanAttn_TrainAttn_Processor:
         return attn.to_out[1](attn.to_out[0](o.transpose(1, 2).flatten(2)))
 
 
-def heads_module_watched(m) -> bool:
+def _module_watched(m) -> bool:
     """Something waits for a call of the module: hooks, its own or every module's, or a forward set on it."""
     return "forward" in m.__dict__ or any(getattr(torch.nn.modules.module, n, None) for n in heads.GLOBAL_HOOKS) or \
         any(getattr(m, n) for n in heads.MODULE_HOOKS)

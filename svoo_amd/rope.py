@@ -156,7 +156,9 @@ def axis_rope(x: torch.Tensor, axes: Sequence[int], *, grid: Optional[Sequence[i
 
     ``norm``: ``"none"``, ``"row"`` (over all heads of a token, Wan's) or ``"head"`` (HunyuanVideo's), with ``weight``
     ``[H * D]`` or ``[D]`` if any.  Differentiable in x and weight, once."""
-    _lib.refuse_unseen("axis_rope", x, weight)
+    _lib.refuse_unseen("axis_rope", x, weight, positions if isinstance(positions, torch.Tensor) else None)
+    if isinstance(positions, torch.Tensor) and _lib.wants_grad(positions):
+        raise RuntimeError("axis_rope has no gradient for positions: detach them")
     eps = float(eps)
     if _lib.wants_grad(x, weight):
         args = tuple(axes), grid if grid is None else tuple(grid), start if start is None else tuple(start), \

@@ -322,3 +322,28 @@ def test_captured_and_replayed(gpu):
         torch.cuda.synchronize()
         for a, b in zip(out, step(*args)):
             assert torch.equal(a, b)
+
+
+def test_offsets_past_32_bits(gpu):
+    """Rows 16 MB apart, and batch entries further: operands in a buffer of 12 GB give the bits of packed ones."""
+    from svoo_amd import dense
+
+    q, k, v, dy = (t.contiguous() for t in make(23, 2, 1, 1, 90, 350, 64, BF, gpu))
+    want = dense.dense_attention_fwd(q, k, v)
+    grads = dense.dense_attention_bwd(dy, q, k, v, *want)
+    row = (1 << 23) - 8
+    buffer = torch.empty(2 * 350 * row, dtype=BF, device=gpu)
+    # every operand has 64 columns of its own in each row
+    apart = [buffer.as_strided(t.shape, (350 * row, 0, row, 1), 64 * i).copy_(t) for i, t in enumerate((q, k, v, dy, want[0]))]
+    got = dense.dense_attention_fwd(*apart[:3])
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    for a, b in zip(dense.dense_attention_bwd(apart[3], *apart[:3], apart[4], want[1], want[2]), grads):
+        assert torch.equal(a, b)
+
+
+def test_rows_too_far_apart_are_copied(gpu):
+    from svoo_amd import dense
+
+    q, k, v, _ = (t.contiguous() for t in make(24, 1, 1, 1, 20, 30, 64, BF, gpu))
+    far = torch.empty(30 << 23, dtype=BF, device=gpu).as_strided(k.shape, (0, 0, 1 << 23, 1)).copy_(k)
+    assert torch.equal(dense.dense_attention(q, far, v), dense.dense_attention(q, k, v))

@@ -252,3 +252,59 @@ def test_captured_and_replayed(gpu):
         torch.cuda.synchronize()
         for a, b in zip(out, step()):
             assert torch.equal(a, b)
+
+
+def test_offsets_past_32_bits(gpu):
+    from svoo_amd import norm
+
+    g, (x, branch, dh, dy) = make(16, 3, 4, 96, torch.bfloat16, gpu)
+    ps = [param(g, 3, 96, "own", torch.float32, gpu) for _ in range(3)]
+    kw = dict(zip(("gate", "scale", "shift"), ps))
+    h, y, mean, rstd = norm.residual_norm_fwd(x, branch, **kw)
+    grads = norm.residual_norm_bwd(dh, dy, h, branch, mean, rstd, **kw)
+    step = (1 << 31) + 24
+    buffer = torch.empty(2 * step + 5000, dtype=torch.bfloat16, device=gpu)
+    far = [buffer.as_strided(x.shape, (step, 96, 1), 1000 * i).copy_(t) for i, t in enumerate((x, branch, dh, dy))]
+    got = norm.residual_norm_fwd(*far[:2], **kw)
+    assert all(torch.equal(a, b) for a, b in zip(got, (h, y, mean, rstd)))
+    for a, b in zip(norm.residual_norm_bwd(far[2], far[3], h, far[1], mean, rstd, **kw), grads):
+        assert torch.equal(a, b)
+
+
+def test_a_tensor_that_is_both_stream_and_branch(gpu):
+    from svoo_amd import norm
+
+    g, (x, _, dh, dy) = make(17, 2, 30, 64, torch.float32, gpu)
+    leaf = x.detach().requires_grad_()
+    h, y = norm.residual_norm(leaf, leaf)
+    both = torch.autograd.grad([h, y], leaf, [dh, dy])[0]
+    h2, _, mean, rstd = norm.residual_norm_fwd(x, x)
+    dx, db = norm.residual_norm_bwd(dh, dy, h2, x, mean, rstd)[:2]
+    assert torch.equal(h, h2) and torch.equal(both, dx + db)
+    assert torch.equal(norm.gated_residual(x, x), 2 * x)
+
+
+def test_streams(gpu):
+    """Calls on other streams, two at a time, with workspaces of their own."""
+    from svoo_amd import norm, rope
+
+    sets = [make(i, 2, 500, 768, torch.bfloat16, gpu)[1] for i in (18, 19)]
+
+    def step(x, branch, dh, dy):
+        h, y, mean, rstd = norm.residual_norm_fwd(x, branch)
+        x4 = x.view(2, 500, 6, 128)
+        w = torch.ones(768, device=gpu)
+        return [h, y, *norm.residual_norm_bwd(dh, dy, h, branch, mean, rstd)[:2],
+                *rope.axis_rope_bwd(dy.view_as(x4), x4, (128,), grid=(500,), norm="row", weight=w)]
+
+    want = [step(*s) for s in sets]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(gpu) for _ in sets]
+    got = []
+    for st, s in zip(streams, sets):
+        st.wait_stream(torch.cuda.current_stream(gpu))
+        with torch.cuda.stream(st):
+            got.append(step(*s))
+    torch.cuda.synchronize()
+    for a, b in zip(got, want):
+        assert all(torch.equal(p, q) for p, q in zip(a, b))

@@ -233,3 +233,18 @@ def test_captured_and_replayed(gpu):
         torch.cuda.synchronize()
         for a, b in zip(out, step()):
             assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("norm", ["row", "head", "none"])
+def test_offsets_past_32_bits(gpu, norm):
+    from svoo_amd import rope
+
+    x, dy, w = make(19, 3, 5, 2, 64, torch.bfloat16, gpu, norm)
+    kw = dict(norm=norm, weight=w, grid=(5,))
+    want, grads = rope.axis_rope(x, (64,), **kw), rope.axis_rope_bwd(dy, x, (64,), **kw)
+    step = (1 << 31) + 24
+    buffer = torch.empty(2 * step + 5000, dtype=torch.bfloat16, device=gpu)
+    far, far_dy = (buffer.as_strided(x.shape, (step, 128, 64, 1), at).copy_(t) for at, t in ((0, x), (2000, dy)))
+    assert torch.equal(rope.axis_rope(far, (64,), **kw), want)
+    for a, b in zip(rope.axis_rope_bwd(far_dy, far, (64,), **kw), grads):
+        assert b is None or torch.equal(a, b)

@@ -203,6 +203,8 @@ def test_rope_refuses_in_python(launches):
     for shape in ((6,), (5, 1), (3, 6, 1), (6, 2)):
         with pytest.raises(ValueError, match="positions: shape"):
             rope.axis_rope(x, (64,), positions=torch.zeros(shape, dtype=torch.int32))
+    with pytest.raises(RuntimeError, match="no gradient for positions"):
+        rope.axis_rope(x, (64,), positions=torch.zeros(6, 1, requires_grad=True))
     for norm, n in (("row", 64), ("head", 192), ("none", 64)):
         with pytest.raises(ValueError, match="weight: shape"):
             rope.axis_rope(x, (64,), positions=pos, norm=norm, weight=torch.ones(n))
