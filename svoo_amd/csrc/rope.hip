@@ -8,6 +8,9 @@
 // Lanes: ceil(D / 8) of them hold a head, four pairs each, and a wave as many whole heads as fit: a lane's columns lie at the
 // same place of every head it sees, so its angles are those of one place.  Angles are whole turns in doubles (a position of
 // 10^5 times a rate keeps 30 bits behind the point), reduced to an eighth of a turn and rounded to fp32 there.
+//
+// bf16, 128 channels, a norm over the row: 32760 x 12 heads 37 us (5.4 TB/s) forward and 61 (4.9) backward, 75600 x 40 heads
+// 295 (5.2) and 450 (5.2); backward straight after forward, whose results are still being written out of the caches, 530.
 #include <algorithm>
 #include <type_traits>
 
@@ -172,6 +175,9 @@ __device__ __forceinline__ int unit_col(int u, int e, int half) {  // within the
 // ---------------------------------------------------------------- a norm over the whole row: one wave or four a token
 // Angles: each lane turns one pair a row (two or more where heads have over 128 channels) and leaves cos and sin in LDS for
 // all heads; the next row's while this one's sums cross the lanes.
+// A wave takes a row alone where its registers hold it, else the block's four share one and meet in LDS: 32760 x 12 heads 37
+// us forward and 61 backward alone, 73 and 133 shared; 75600 x 40 heads forward 297 and 306.  Backward, 40 heads alone leave
+// two waves a SIMD: 590 us of 540 shared, with a forward pass in front.
 template <int T, int WPR, int NC, bool kHalves, bool kGrad>
 __global__ void __launch_bounds__(256) rope_row_kernel(RopeArgs a) {
   constexpr int kGroups = 4 / WPR, kTpr = WPR * kWave;  // rows of a block at a time
