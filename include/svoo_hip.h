@@ -386,7 +386,7 @@ int svoo_axis_rope_bwd(const void* dy, long long dy_batch_stride, long long dy_r
 /* ---------------------------------------------------------------------------------------------
  * Dense attention with a backward pass (no reference counterpart: the reference calls the framework's).  q [batch][heads][sq][d],
  * k and v [batch][kv_heads][sk][d] by strides in elements, columns contiguous, rows at 16-byte addresses (strides in multiples
- * of 8); type 0 bf16, 1 fp16; d a multiple of 8 up to 128; heads a multiple of kv_heads; scale above 0.  q_lens and k_lens
+ * of 8, rows fewer than 2^23 elements apart); type 0 bf16, 1 fp16; d a multiple of 8 up to 128; heads a multiple of kv_heads; scale above 0.  q_lens and k_lens
  * (device int32 [batch] or NULL, clamped to 0..sq and 0..sk): rows behind them are not read and have o = 0 and no gradient.
  *   svoo_dense_attention_fwd: o [batch][sq][heads][d] contiguous, o_rest (optional) what its rounding left, in the same type
  *     and layout, for a backward pass of full accuracy, and lse [batch][heads][sq] (fp32, -inf for queries without keys).

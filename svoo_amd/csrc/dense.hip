@@ -280,7 +280,9 @@ __global__ void __launch_bounds__(256) dense_join_kernel(DenseArgs a) {
 }
 
 // Shares of the contracted length for a launch of `blocks` blocks that each walk over `units` tiles: the fewest rounds of 256
-// resident blocks times tiles, with two tiles' time for writing and joining partial results.
+// resident blocks times tiles, with two tiles' time for writing and joining partial results.  With shares and in one: a query
+// over 12 x 32760 keys 43 and 577 us; dk and dv of 12 x 512 keys from 32760 queries 260 and 1750, of 3 x 2 x 771 keys from 4
+// heads of 1037 queries 36 and 181; nothing to win with 12 x 128 blocks (two shares 145 us, one 154).
 int dense_shares(long long blocks, long long units, long long bytes) {
   long long best = 1, cost = (blocks + 255) / 256 * units;
   for (long long s = 2; s <= 256 && s * 4 <= units && s * bytes <= (256ll << 20); ++s) {
