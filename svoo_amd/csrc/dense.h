@@ -165,6 +165,18 @@ __device__ __forceinline__ unsigned xcd_block(unsigned bid, unsigned total) {
   return (bid % 8) * each + bid / 8;
 }
 
+// Where four rounds of blocks or more walk over few tiles, the first round's blocks (one a CU) start apart, over about the time
+// of a block (15 us at most): else all of them read their rows at the same time, then all compute, and so to the end.  bf16,
+// 128 columns, forward and dq without and with it: 12 x 22000 x 512 105 and 95, 120 and 108 us; 12 x 32760 x 512 133 and 128,
+// 181 and 168, x 64 67 and 63, 79 and 77, x 1024 212 and 211, 301 and 294; 64 columns, 16 x 32760 x 512 115 and 116, 143 and
+// 142.  Above 16 tiles a walk nothing is won (12 x 32760 x 4096 711 and 717 us), and delays twice as long lost 5% at 1024.
+template <int DP>
+__device__ __forceinline__ void start_apart(unsigned total, int ntiles) {
+  if (blockIdx.x >= 256 || total < 1024 || ntiles > 16) return;
+  const int n = (int)blockIdx.x / 8 * min(ntiles, 8) * DP / 128;
+  for (int i = 0; i < n; ++i) __builtin_amdgcn_s_sleep(2);
+}
+
 // Four values to 16 bits, and what that leaves of them.
 template <int T>
 __device__ __forceinline__ uint2 pack4(f32x4_t v) { return make_uint2(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3])); }

@@ -10,7 +10,7 @@ constexpr int kFwdWaves = 8, kFwdQ = kFwdWaves * 32, kFwdK = 64;
 // S(t+1) = K(t+1) Q^T} and the softmax of the next, so that matrix and vector units are busy at the same time.
 //
 // What bounds it: the chip's power.  12 heads of 32760 x 32760, 128 columns, take 5.55 ms (1.19 PFLOP/s) at 2.05 GHz, matrix
-// units busy in 51% of the cycles and no LDS bank conflicts; on zeros, at 2.4 GHz, 4.55 ms.  12 x 32760 x 512: 137 us (0.75
+// units busy in 51% of the cycles and no LDS bank conflicts; on zeros, at 2.4 GHz, 4.55 ms.  12 x 32760 x 512: 128 us (0.81
 // PFLOP/s), a third of it the ends of so short a walk; one query over 12 x 32760 keys: 38 us (5.3 TB/s).  Blocks of four
 // waves, two of them on a CU, overlap these ends but read K and V twice as often: 142 and 148 us with 512 keys, 6.3 ms with
 // 32760.  Walking over several query tiles in one block spills (7.7 ms, and 6.8 with chains of tiles).
@@ -52,6 +52,7 @@ dense_fwd_kernel(DenseArgs a) {
     return;
   }
   const bool active = q0 + wave * 32 < q_len;  // uniform over the wave
+  start_apart<DP>(total, ntiles);
   u32x4_t qop[kS];
   load_operand<DP, kFull>(a.q.p + (long long)b * a.q.batch + (long long)head * a.q.head + (long long)min(row, q_len - 1) * a.q.row, a.d,
                    h, qop);

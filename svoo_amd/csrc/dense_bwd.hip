@@ -131,7 +131,8 @@ __device__ __forceinline__ void alternate(int tiles, bool group_b, bool active, 
 // dq.  A block: 8 waves of 32 queries, one per lane; K and V tiles of 64 keys double buffered in LDS.  S^T = K Q^T and
 // dP^T = V dO^T leave a query's 16 keys in its lane, and dS^T is at once the operand of dQ^T += K^T dS^T.
 // What bounds it: power.  12 x 32760 x 32760 x 128 takes 8.4 ms (1.18 PFLOP/s of three products) at 2.10 GHz with the matrix
-// units busy in 51% of the cycles; on zeros 7.2.  12 x 32760 x 512: 195 us.
+// units busy in 51% of the cycles; on zeros 7.2.  12 x 32760 x 512: 168 us.  Making
+// delta here costs what its kernel does (245 us of both, 249): its loads too come at the blocks' starts.
 template <int T, int DP, bool kFull>
 __global__ void __launch_bounds__(kBwdWaves * kWave) __attribute__((amdgpu_waves_per_eu(2, 2)))
 dense_dq_kernel(DenseArgs a) {
@@ -153,6 +154,7 @@ dense_dq_kernel(DenseArgs a) {
   for (int db = 0; db < kB; ++db) acc[db] = f32x16_t{};
   float e16 = 0.0f;
   if (ntiles > 0) {  // uniform
+    start_apart<DP>(total, ntiles);
     if (T == kDenseF16) e16 = f16_exponent(a, b, kv, scratch);
     const float by = T == kDenseF16 ? __builtin_amdgcn_exp2f(e16) : 1.0f;
     const int r = min(row, q_len - 1);
