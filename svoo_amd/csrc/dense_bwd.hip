@@ -132,7 +132,7 @@ __device__ __forceinline__ void alternate(int tiles, bool group_b, bool active, 
 // dP^T = V dO^T leave a query's 16 keys in its lane, and dS^T is at once the operand of dQ^T += K^T dS^T.
 // What bounds it: power.  12 x 32760 x 32760 x 128 takes 8.4 ms (1.18 PFLOP/s of three products) at 2.10 GHz with the matrix
 // units busy in 51% of the cycles; on zeros 7.2.  12 x 32760 x 512: 168 us.  Making
-// delta here costs what its kernel does (245 us of both, 249): its loads too come at the blocks' starts.
+// delta here in place of its kernel gained 2% of the two there: its loads too come at the blocks' starts.
 template <int T, int DP, bool kFull>
 __global__ void __launch_bounds__(kBwdWaves * kWave) __attribute__((amdgpu_waves_per_eu(2, 2)))
 dense_dq_kernel(DenseArgs a) {

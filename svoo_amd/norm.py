@@ -282,8 +282,8 @@ def _residual_forward(c: _Residual, branch, normed: bool, stats: bool):
     """``(h, y or None, statistics [2, rows] or None)``."""
     at, *strides = c.rows_of(c.x, "x")
     b_args = c.rows_of(branch, "branch")
-    h = torch.empty(c.shape, dtype=c.x.dtype, device=c.device)
-    y = torch.empty(c.shape, dtype=c.x.dtype, device=c.device) if normed else None
+    h = torch.empty_like(c.x, memory_format=torch.contiguous_format)
+    y = torch.empty_like(c.x, memory_format=torch.contiguous_format) if normed else None
     rows = c.batch * c.rows
     st = torch.empty((2, rows), dtype=torch.float32, device=c.device) if stats else None
     mean = st.data_ptr() if stats else None
@@ -296,10 +296,10 @@ def _residual_backward(c: _Residual, dh, dy, h, branch, mean, rstd, needs):
     """``(dx, dbranch, dgate, dweight, dbias)`` as ``needs`` says; dy, h and the statistics are None for a residual alone."""
     params = c.params
     want = [p is not None and bool(n) for p, n in zip(params, needs[2:])]
-    new = [torch.empty(c.shape, dtype=c.x.dtype, device=c.device) if n else None for n in needs[:2]]
+    new = [torch.empty_like(c.x, memory_format=torch.contiguous_format) if n else None for n in needs[:2]]
     if c.batch * c.rows == 0:
         return (*new, *(torch.zeros_like(p) if w else None for p, w in zip(params, want)))
-    sums = [torch.empty(p.shape, dtype=p.dtype, device=c.device) if w else None for p, w in zip(params, want)]
+    sums = [torch.empty_like(p, memory_format=torch.contiguous_format) if w else None for p, w in zip(params, want)]
     if not any(needs[:2]) and not any(want):
         return (*new, *sums)
     size, ws = 0, None

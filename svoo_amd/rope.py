@@ -96,7 +96,7 @@ class _Call:
 
 
 def _forward(c: _Call, x, eps):
-    y = torch.empty(c.shape, dtype=x.dtype, device=c.device)
+    y = torch.empty_like(x, memory_format=torch.contiguous_format)
     at, *strides = c.rows_of(x)
     _lib.launch(c.device, "svoo_axis_rope_fwd", at, c.kind, *strides, *c.shape, c.norm, *c.w_args, eps, *c.where, y.data_ptr())
     return y
@@ -105,7 +105,7 @@ def _forward(c: _Call, x, eps):
 def _backward(c: _Call, dy, x, eps, needs):
     if _lib.elem_type(dy, "dy") != c.kind or dy.shape != c.shape or dy.device != c.device:
         raise ValueError(f"dy: {dy.dtype} {tuple(dy.shape)} on {dy.device}, x {x.dtype} {tuple(c.shape)} on {c.device}")
-    dx = torch.empty(c.shape, dtype=x.dtype, device=c.device) if needs[0] else None
+    dx = torch.empty_like(dy, memory_format=torch.contiguous_format) if needs[0] else None
     need_w = needs[1] and c.weight is not None
     if dy.numel() == 0:
         return dx, torch.zeros_like(c.weight) if need_w else None
