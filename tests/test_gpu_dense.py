@@ -347,3 +347,20 @@ def test_rows_too_far_apart_are_copied(gpu):
     q, k, v, _ = (t.contiguous() for t in make(24, 1, 1, 1, 20, 30, 64, BF, gpu))
     far = torch.empty(30 << 23, dtype=BF, device=gpu).as_strided(k.shape, (0, 0, 1 << 23, 1)).copy_(k)
     assert torch.equal(dense.dense_attention(q, far, v), dense.dense_attention(q, k, v))
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("sq,sk", [(100, 1500), (3, 9000), (600, 4000), (1700, 130)])
+def test_lengths_that_leave_shares_empty(gpu, sq, sk, dtype):
+    """A long axis is split into a few shares or many, of which a short sequence fills the first ones only."""
+    say("shares", sq, sk, dtype)
+    q, k, v, dy = make(25, 4, 2, 1, sq, sk, 64, dtype, gpu)
+    check(q, k, v, dy, q_lens=lens([sq, sq, (sq + 1) // 2, 0], gpu), k_lens=lens([sk, 65, 0, sk], gpu))
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("d,sk", [(64, 70), (128, 600), (40, 1)])
+def test_many_blocks(gpu, d, sk, dtype):
+    """More blocks than a few rounds of all CUs, of one tile of queries each."""
+    say("many blocks", d, sk, dtype)
+    check(*make(26, 5, 230, 46, 9, sk, d, dtype, gpu))
