@@ -2,7 +2,7 @@
 //   S = scale q k^T over the keys of a sequence,  L = logsumexp(S),  P = exp(S - L),  o = P v
 //   backward  D = rowsum(do o),  dP = do v^T,  dS = P (dP - D),  dv = P^T do,  dq = scale dS k,  dk = scale dS^T q
 // Queries from a sequence's length on have o = 0 and no gradient, keys from theirs on take no part; a query without keys has
-// o = 0 and L = -inf.
+// o = 0 and L = -inf.  A score of -inf has P = 0; a query that has keys but no other scores has no P: o and L are NaN.
 //
 // Every product is a 32 x 32 x 16 matrix instruction whose accumulator is the next product's operand as it lies: scores come
 // out with one query (or key) per lane and 16 of the other side in its registers, which is the operand of the product that
@@ -59,6 +59,9 @@ struct DenseArgs {
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
+// A running maximum starts at the lowest number: from -inf, a tile whose scores are all -inf would have P = exp(-inf + inf), and
+// the row would be NaN for good, whatever follows.
+constexpr float kLowest = -3.4028234663852886e38f;
 constexpr int kNormRows = 256;  // rows that share a maximum
 // fp16's P runs to 2^14, so that 1 / N of a long even row is a normal number
 constexpr float kF16PShift = 14.0f;
@@ -74,6 +77,10 @@ template <int T>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   if (T == kDenseBf16) return cvt_pk_bf16(lo, hi);
   return (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)lo) | ((uint32_t)__builtin_bit_cast(uint16_t, (_Float16)hi) << 16);
+}
+// L of a row with keys, from its maximum and sum; NaN without a finite score.
+__device__ __forceinline__ float row_lse(float m, float l) {
+  return l > 0.0f ? (m + __builtin_amdgcn_logf(l)) * kLn2 : __builtin_nanf("");
 }
 // c plus a pair's two values (P rounded: o is divided by the sum of what multiplied v, so that its weights sum to 1)
 template <int T>

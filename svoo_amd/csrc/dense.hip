@@ -63,7 +63,7 @@ dense_fwd_kernel(DenseArgs a) {
   f32x16_t acc[kB], sacc[2];
 #pragma unroll
   for (int db = 0; db < kB; ++db) acc[db] = f32x16_t{};
-  float m_run = -INFINITY, l_run = 0.0f, w_run = 0.0f;  // the maximum, the sum of P, and the sum of P as it multiplies V
+  float m_run = kLowest, l_run = 0.0f, w_run = 0.0f;  // the maximum, the sum of P, and the sum of P as it multiplies V
   u32x4_t pop[2][2];
   const float sl = a.scale_log2;
   const int last = k_len - 1;
@@ -220,7 +220,7 @@ dense_fwd_kernel(DenseArgs a) {
   if (row < q_len) {
     const size_t to = out0 + (size_t)row * a.heads * a.d;
     store_row16<T, DP, kFull>(a.out + to, a.rest != nullptr ? a.rest + to : nullptr, acc, a.d, h, 1.0f / w_run);
-    if (h == 0) a.lse[stat + row] = (m_run + __builtin_amdgcn_logf(l_run)) * kLn2;
+    if (h == 0) a.lse[stat + row] = row_lse(m_run, l_run);
   } else {
     zero_row();
   }
@@ -244,7 +244,7 @@ __global__ void __launch_bounds__(256) dense_join_kernel(DenseArgs a) {
 #pragma unroll 4
     for (int s = slice; s < a.splits; s += kJoinSlices) {
       const float4 ml = a.part_ml[s * rows + at];
-      if (ml.x == -INFINITY && !(ml.y != ml.y)) continue;  // an empty share wrote no row
+      if (ml.x == -INFINITY) continue;  // an empty share wrote no row
       const float w = __builtin_amdgcn_exp2f(ml.x - m);
       l = fmaf(ml.y, w, l);
       lw = fmaf(ml.z, w, lw);
@@ -264,20 +264,20 @@ __global__ void __launch_bounds__(256) dense_join_kernel(DenseArgs a) {
 #pragma unroll
   for (int i = 0; i < kJoinSlices; ++i) {
     const int j = threadIdx.x + i * per_row;
-    if (s_m[j] == -INFINITY && !(s_l[j] != s_l[j])) continue;
+    if (s_m[j] == -INFINITY) continue;
     const float w = __builtin_amdgcn_exp2f(s_m[j] - m);
     l = fmaf(s_l[j], w, l);
     lw = fmaf(s_w[j], w, lw);
     o += s_o[j] * w;
   }
-  const bool some = l > 0.0f || l != l;
+  const bool some = m > -INFINITY;  // keys: the lowest maximum of a share with any is kLowest
   const int row = (int)(at % a.sq), bh = (int)(at / a.sq);
   const size_t to = ((size_t)(bh / a.heads) * a.sq + row) * a.heads * a.d + (size_t)(bh % a.heads) * a.d + 4 * c;
   o *= some ? 1.0f / lw : 0.0f;
   const uint2 w = pack4<T>(o);
   *(uint2*)(a.out + to) = w;
   if (a.rest != nullptr) *(uint2*)(a.rest + to) = pack4<T>(rest4<T>(o, w));
-  if (c == 0) a.lse[at] = some ? (m + __builtin_amdgcn_logf(l)) * kLn2 : -INFINITY;
+  if (c == 0) a.lse[at] = some ? row_lse(m, l) : -INFINITY;
 }
 
 // Shares of the contracted length for a launch of `blocks` blocks that each walk over `units` tiles: the fewest rounds of 256

@@ -161,7 +161,8 @@ def dense_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, scale:
 
     ``q_lens`` and ``k_lens`` (int32 ``[B]``, on the GPU; read there, values outside 0..S count as the nearest) are the valid
     rows of each batch entry: what lies behind them is not read, whatever it holds, results there are 0, and so are the
-    results of queries without keys.  The result is ``[B, H, Sq, D]``, contiguous as ``[B, Sq, H, D]``.  Differentiable in
+    results of queries without keys.  Keys whose score is -inf (a channel that masks them) have the probability 0, wherever they
+    lie; a query whose every score is -inf is NaN.  The result is ``[B, H, Sq, D]``, contiguous as ``[B, Sq, H, D]``.  Differentiable in
     q, k and v, once."""
     _lib.refuse_unseen("dense_attention", q, k, v)
     if _lib.wants_grad(q, k, v):
