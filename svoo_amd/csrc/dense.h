@@ -7,8 +7,8 @@
 // Every product is a 32 x 32 x 16 matrix instruction whose accumulator is the next product's operand as it lies: scores come
 // out with one query (or key) per lane and 16 of the other side in its registers, which is the operand of the product that
 // contracts that side, up to the order of the contracted positions; the other operand is read from LDS in the same order by
-// gfx950's transposing read.  Rows behind a sequence's end are read as its last row (finite times P = 0), columns behind the
-// head dim as zeros.
+// gfx950's transposing read.  Rows behind a sequence's end are read as its last row, columns behind the head dim as zeros; rows
+// of v and do there, which are multiplied by P = 0, become zeros too (an infinite last row would make 0 times inf).
 #pragma once
 
 #include <algorithm>
@@ -125,6 +125,15 @@ __device__ __forceinline__ void tile_dma(const uint16_t* base, long long row_str
     const uint32_t n = w * kIt + j, c = chunk ^ (DP == 128 ? n & 3 : (n & 1) << 2);
     if (kFull || c * 8 < (uint32_t)d) lds_dma16(from + (__umul24(min(n * kEach + row, (uint32_t)most), step) + c * 16), tile + n * 64 * 8);
   }
+}
+// Rows n .. of a tile as zeros, each wave those that it copied, once its copies are there.
+template <int DP, int kRows, int kWaves>
+__device__ __forceinline__ void tile_end(uint16_t* tile, int n, int w, int lane) {
+  constexpr int kEach = kRows / kWaves * DP / 8;  // 16-byte chunks of a wave
+  w = __builtin_amdgcn_readfirstlane(w);
+#pragma unroll
+  for (int i = 0; i < kEach; i += 64)
+    if (w * kEach + i + lane >= n * (DP / 8)) ((u32x4_t*)tile)[w * kEach + i + lane] = u32x4_t{0, 0, 0, 0};
 }
 // Tiles with columns that no copy fills, once: zeros.
 template <int DP, int kThreads, int kElems>

@@ -70,6 +70,12 @@ dense_fwd_kernel(DenseArgs a) {
   auto dma = [&](const DenseRows& m, const uint16_t* base, int t, uint16_t* to) __attribute__((always_inline)) {
     tile_dma<DP, kFull, kFwdK, 4>(base, m.row, (t0 + t) * kFwdK, last, a.d, to, wg, lane);
   };
+  // the copied V(t) is there, its rows behind the last key zeros
+  const int ragged = k_len % kFwdK != 0 ? all - 1 - t0 : -1;  // the tile with such rows
+  auto v_there = [&](int t, uint16_t* tile) __attribute__((always_inline)) {
+    __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    if (__builtin_expect(t == ragged, 0)) tile_end<DP, kFwdK, 4>(tile, k_len % kFwdK, wg, lane);
+  };
   auto scores = [&](const uint16_t* kt) __attribute__((always_inline)) {
     sacc[0] = f32x16_t{};
     sacc[1] = f32x16_t{};
@@ -178,7 +184,7 @@ dense_fwd_kernel(DenseArgs a) {
     dma(a.k, kb, 0, k_s[0]);
     dma(a.v, vb, 0, v_s[0]);
     dma(a.k, kb, 1, k_s[1]);
-    __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    v_there(0, v_s[0]);
   }
   __syncthreads();
   if (active) scores(k_s[0]);
@@ -202,7 +208,7 @@ dense_fwd_kernel(DenseArgs a) {
           if (active && t + u + 1 < ntiles) vphase(t + u + 1);
         } else {
           if (active) mphase(v_s[u], k_s[u ^ 1]);
-          __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory");
+          v_there(t + u + 1, v_s[u ^ 1]);
         }
         __syncthreads();
       }

@@ -299,9 +299,11 @@ dense_dkv_kernel(DenseArgs a) {
     // L and D of a tile: group B's first 128 threads, a value each, loaded with the copies and left in LDS after them
     float stat = 0.0f;
     const int si = tid - 4 * kWave;
+    int left = kBwdTile;  // queries from the copied tile's first on
     auto place = [&](int u) __attribute__((always_inline)) { return u / 2 % 2 * kElems + u % 2 * 32 * DP; };
     auto copy = [&](int t) __attribute__((always_inline)) {
       const int head = kv * a.group + (t0 + t) / qt, q0 = (t0 + t) % qt * kBwdTile;
+      left = q_len - q0;
       tile_dma<DP, kFull, kBwdTile, 4>(a.q.p + (long long)b * a.q.batch + (long long)head * a.q.head, a.q.row, q0, last, a.d,
                                        q_s + t % 2 * kElems, wg, lane);
       tile_dma<DP, kFull, kBwdTile, 4>(a.dy.p + (long long)b * a.dy.batch + (long long)head * a.dy.head, a.dy.row, q0, last, a.d,
@@ -315,6 +317,7 @@ dense_dkv_kernel(DenseArgs a) {
     };
     auto wait = [&](int t) __attribute__((always_inline)) {
       __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      if (__builtin_expect(left < kBwdTile, 0)) tile_end<DP, kBwdTile, 4>(d_s + t % 2 * kElems, left, wg, lane);
       if (si < kBwdTile) stat_s[t % 2][0][si] = stat == -INFINITY ? -INFINITY : fmaf(-stat, kLog2e, kShift);
       else if (si < 2 * kBwdTile) stat_s[t % 2][1][si - kBwdTile] = -stat * by;
     };
