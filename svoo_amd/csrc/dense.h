@@ -63,8 +63,12 @@ constexpr float kLn2 = 0.6931471805599453f;
 // the row would be NaN for good, whatever follows.
 constexpr float kLowest = -3.4028234663852886e38f;
 constexpr int kNormRows = 256;  // rows that share a maximum
-// fp16's P runs to 2^14, so that 1 / N of a long even row is a normal number
+// fp16's P runs to 2^14 in the backward pass, so that 1 / N of a long even row is a normal number
 constexpr float kF16PShift = 14.0f;
+// and in the forward pass from 2^12 of a running maximum to the type's end: with all its bits to 2^-26 of the largest, in steps of
+// 2^-36 below.  With P = 1 at the maximum, keys 14 bits below it lost bits and those 25 below it were lost, which is all of o
+// where the largest one's value is 0 (8192 such keys 17 nats below: o half of what it is).
+constexpr float kF16Top = 12.0f;
 
 typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
 

@@ -7,8 +7,10 @@ call gives the same bits.
 
 Tensors are ``[B, H, S, D]`` in bf16 or fp16 on the GPU, with any strides (rows that are not contiguous or not at 16-byte
 addresses, and head dims that are no multiple of 8, are copied first); D is at most 128.  Scores, statistics and sums are
-fp32; probabilities and their gradients are rounded to the tensors' type before they are multiplied (fp16 by powers of two
-that keep them within its range).  fp32 tensors are refused: they would lose two thirds of their digits.
+fp32; probabilities and their gradients are rounded to the tensors' type before they are multiplied.  fp16's are multiplied by
+powers of two: probabilities keep all their bits down to 2^-26 of the largest of a row (18 below the highest score) in the
+forward pass and to 2^-28 in the backward pass, and lose them over the ten bits below.  fp32 tensors are refused: they would
+lose two thirds of their digits.
 
 :func:`dense_attention` is differentiable; :func:`dense_attention_fwd` and :func:`dense_attention_bwd` are its two passes as
 plain calls, for programs that capture a training step into a graph.
