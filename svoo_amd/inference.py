@@ -168,22 +168,33 @@ def replace_wan_attention_trainable(pipe, height: int, width: int, num_frames: i
     """Install dense attention with gradients (:class:`svoo_amd.processor.WanAttn_TrainAttn_Processor`) in ``attn1`` and
     ``attn2`` of every block of a Wan pipeline's transformers, for training on clips of this size.
 
-    The transformer is bf16 or fp16, with head dims up to 128 and no image branch (``ValueError`` before the first change).
+    Refused before the first change (``ValueError``): in either transformer an odd head dim or one above 128, an image branch, or
+    an attention that takes no processor; patches of another size in the second.  Element types are seen at the first call,
+    which takes bf16 and fp16 projections (an fp32 transformer's under autocast) and raises ``TypeError`` for others.
     ``theta`` is the rotary base, 10000 for every Wan model.  Returns the processors."""
-    patch = pipe.transformer.config.patch_size
+    name = "replace_wan_attention_trainable"
+    patch = tuple(pipe.transformer.config.patch_size)
     frames, _ = wan_token_geometry(pipe, height, width, num_frames)
     mod_h, mod_w = (pipe.vae_scale_factor_spatial * p for p in patch[1:])
-    d = pipe.transformer.config.attention_head_dim
-    if not 1 <= d <= 128 or d % 2:
-        raise ValueError(f"replace_wan_attention_trainable: head dim {d}")
-    blocks = [b for t in (pipe.transformer, getattr(pipe, "transformer_2", None)) if t is not None for b in t.blocks]
-    layers = [a for b in blocks for a in (b.attn1, getattr(b, "attn2", None)) if a is not None]
-    if any(getattr(a, "add_k_proj", None) is not None for a in layers):
-        raise ValueError("replace_wan_attention_trainable: an image branch")
-    hw = 2 * (d // 6)
+    layers = []
+    for t in (pipe.transformer, getattr(pipe, "transformer_2", None)):
+        if t is None:
+            continue
+        d = t.config.attention_head_dim
+        if not 1 <= d <= 128 or d % 2:
+            raise ValueError(f"{name}: head dim {d}")
+        if tuple(t.config.patch_size) != patch:
+            raise ValueError(f"{name}: patches of {tuple(t.config.patch_size)} in the second transformer, {patch} in the first")
+        hw = 2 * (d // 6)
+        for a in (a for b in t.blocks for a in (b.attn1, getattr(b, "attn2", None)) if a is not None):
+            if getattr(a, "add_k_proj", None) is not None:
+                raise ValueError(f"{name}: an image branch")
+            if not hasattr(a, "set_processor"):
+                raise ValueError(f"{name}: an attention without set_processor")
+            layers.append((a, (d - 2 * hw, hw, hw)))
     processors = []
-    for a in layers:
-        a.set_processor(WanAttn_TrainAttn_Processor((frames, height // mod_h, width // mod_w), (d - 2 * hw, hw, hw), theta))
+    for a, axes in layers:
+        a.set_processor(WanAttn_TrainAttn_Processor((frames, height // mod_h, width // mod_w), axes, theta))
         processors.append(a.processor)
     return processors
 
