@@ -67,7 +67,7 @@ constexpr int kNormRows = 256;  // rows that share a maximum
 constexpr float kF16PShift = 14.0f;
 // and in the forward pass from 2^12 of a running maximum to the type's end: with all its bits to 2^-26 of the largest, in steps of
 // 2^-36 below.  With P = 1 at the maximum, keys 14 bits below it lost bits and those 25 below it were lost, which is all of o
-// where the largest one's value is 0 (8192 such keys 17 nats below: o half of what it is).
+// where the largest one's value is 0 (even keys at e^-16 and e^-17 of it: o 8% and 44% too large; at e^-18: o = 0).
 constexpr float kF16Top = 12.0f;
 
 typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
