@@ -19,6 +19,7 @@ single-stream block (layers ``D ..``), the numbering the per-layer profile CSV i
 from __future__ import annotations
 
 import os
+from typing import Optional
 
 import torch
 
@@ -164,14 +165,15 @@ def replace_wan_attention(
     return processors
 
 
-def replace_wan_attention_trainable(pipe, height: int, width: int, num_frames: int, theta: float = 10000.0):
+def replace_wan_attention_trainable(pipe, height: int, width: int, num_frames: int, theta: Optional[float] = None):
     """Install dense attention with gradients (:class:`svoo_amd.processor.WanAttn_TrainAttn_Processor`) in ``attn1`` and
     ``attn2`` of every block of a Wan pipeline's transformers, for training on clips of this size.
 
     Refused before the first change (``ValueError``): in either transformer an odd head dim or one above 128, an image branch, or
     an attention that takes no processor; patches of another size in the second.  Element types are seen at the first call,
     which takes bf16 and fp16 projections (an fp32 transformer's under autocast) and raises ``TypeError`` for others.
-    ``theta`` is the rotary base, 10000 for every Wan model.  Returns the processors."""
+    ``theta`` is the rotary base, each configuration's ``rope_theta`` by default (10000 without one, as in every Wan model).
+    Returns the processors."""
     name = "replace_wan_attention_trainable"
     patch = tuple(pipe.transformer.config.patch_size)
     frames, _ = wan_token_geometry(pipe, height, width, num_frames)
@@ -191,10 +193,10 @@ def replace_wan_attention_trainable(pipe, height: int, width: int, num_frames: i
                 raise ValueError(f"{name}: an image branch")
             if not hasattr(a, "set_processor"):
                 raise ValueError(f"{name}: an attention without set_processor")
-            layers.append((a, (d - 2 * hw, hw, hw)))
+            layers.append((a, (d - 2 * hw, hw, hw), getattr(t.config, "rope_theta", 10000.0) if theta is None else theta))
     processors = []
-    for a, axes in layers:
-        a.set_processor(WanAttn_TrainAttn_Processor((frames, height // mod_h, width // mod_w), axes, theta))
+    for a, axes, base in layers:
+        a.set_processor(WanAttn_TrainAttn_Processor((frames, height // mod_h, width // mod_w), axes, base))
         processors.append(a.processor)
     return processors
 

@@ -71,3 +71,20 @@ def test_fp32_projections_are_refused_at_the_call(monkeypatch):
         attn(x, rotary_emb=dit.rope_tables(cfg, 3, 4, 6, "cpu"))
     with torch.no_grad(), torch.autocast("cpu", torch.bfloat16):
         assert attn(x, rotary_emb=dit.rope_tables(cfg, 3, 4, 6, "cpu")).dtype == torch.bfloat16
+
+
+def test_the_rotary_base_is_the_configurations():
+    from types import SimpleNamespace
+
+    from svoo_amd import dit
+    from svoo_amd.inference import replace_wan_attention_trainable
+
+    cfg = dit.WanDiTConfig(num_attention_heads=2, ffn_dim=64, num_layers=1, text_dim=32, rope_theta=500.0)
+    pipe = dit.make_pipe(cfg, dtype=torch.bfloat16)
+    pipe.transformer_2 = _pipe().transformer
+    assert [p.theta for p in replace_wan_attention_trainable(pipe, 64, 96, 9)] == [500.0] * 2 + [10000.0] * 4
+    assert {p.theta for p in replace_wan_attention_trainable(pipe, 64, 96, 9, theta=7.0)} == {7.0}
+    pipe.transformer_2 = None
+    # a configuration that names no base
+    pipe.transformer.config = SimpleNamespace(patch_size=cfg.patch_size, attention_head_dim=cfg.attention_head_dim)
+    assert {p.theta for p in replace_wan_attention_trainable(pipe, 64, 96, 9)} == {10000.0}
