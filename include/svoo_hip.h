@@ -389,9 +389,11 @@ int svoo_axis_rope_bwd(const void* dy, long long dy_batch_stride, long long dy_r
  * of 8, rows fewer than 2^23 elements apart); type 0 bf16, 1 fp16; d a multiple of 8 up to 128; heads a multiple of kv_heads; scale above 0.  q_lens and k_lens
  * (device int32 [batch] or NULL, clamped to 0..sq and 0..sk): rows behind them are not read and have o = 0 and no gradient.
  *   svoo_dense_attention_fwd: o [batch][sq][heads][d] contiguous, o_rest (optional) what its rounding left, in the same type
- *     and layout, for a backward pass of full accuracy, and lse [batch][heads][sq] (fp32, -inf for queries without keys).
+ *     and layout, for a backward pass of full accuracy, and lse [batch][heads][sq] (fp32, -inf for queries without keys).  Keys
+ *     whose score is -inf have the probability 0; a query whose every score is -inf has o and lse NaN.
  *   svoo_dense_attention_bwd: dq [batch][sq][heads][d], dk and dv [batch][sk][kv_heads][d], contiguous, each optional; the same
- *     call gives the same bits.  The workspace lies at a 16-byte address.
+ *     call gives the same bits.
+ *   Workspaces lie at 16-byte addresses.
  * ------------------------------------------------------------------------------------------- */
 size_t svoo_dense_attention_fwd_workspace_size(int batch, int heads, int sq, int sk, int d);
 int svoo_dense_attention_fwd(const void* q, long long q_batch, long long q_head, long long q_row, const void* k,

@@ -386,7 +386,7 @@ extern "C" int svoo_dense_attention_fwd(const void* q, long long q_batch, long l
   a.tiles = (sq + kFwdQ - 1) / kFwdQ;
   a.splits = fwd_splits(batch, heads, sq, sk, d);
   const size_t need = svoo_dense_attention_fwd_workspace_size(batch, heads, sq, sk, d);
-  SVOO_REQUIRE(need == 0 || (workspace && ws_bytes >= need), SVOO_ERR_WORKSPACE, "%s: workspace of %zu bytes (%zu needed)", name,
+  SVOO_REQUIRE(need == 0 || (workspace && (uintptr_t)workspace % 16 == 0 && ws_bytes >= need), SVOO_ERR_WORKSPACE, "%s: workspace of %zu bytes (%zu needed)", name,
                ws_bytes, need);
   const size_t rows = (size_t)batch * heads * sq;
   a.part = (float*)workspace;
