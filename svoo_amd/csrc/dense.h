@@ -189,7 +189,8 @@ __device__ __forceinline__ unsigned xcd_block(unsigned bid, unsigned total) {
 // of a block (15 us at most): else all of them read their rows at the same time, then all compute, and so to the end.  bf16,
 // 128 columns, forward and dq without and with it: 12 x 22000 x 512 105 and 95, 120 and 108 us; 12 x 32760 x 512 133 and 128,
 // 181 and 168, x 64 67 and 63, 79 and 77, x 1024 212 and 211, 301 and 294; 64 columns, 16 x 32760 x 512 115 and 116, 143 and
-// 142.  Above 16 tiles a walk nothing is won (12 x 32760 x 4096 711 and 717 us), and delays twice as long lost 5% at 1024.
+// 142, 24 x 75600 x 256 280 and 274.  It is kept where it wins nothing, at 64 columns and at 16 tiles, since it costs nothing there.
+// Above 16 tiles a walk nothing is won (12 x 32760 x 4096 711 and 717 us), and delays twice as long lost 5% at 1024.
 template <int DP>
 __device__ __forceinline__ void start_apart(unsigned total, int ntiles) {
   if (blockIdx.x >= 256 || total < 1024 || ntiles > 16) return;

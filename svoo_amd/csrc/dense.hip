@@ -9,11 +9,13 @@ constexpr int kFwdWaves = 8, kFwdQ = kFwdWaves * 32, kFwdK = 64;
 // of a SIMD belong to two groups that alternate, half a step apart, between a tile's matrix work {O += V(t)^T P(t)^T,
 // S(t+1) = K(t+1) Q^T} and the softmax of the next, so that matrix and vector units are busy at the same time.
 //
-// What bounds it: the chip's power.  12 heads of 32760 x 32760, 128 columns, take 5.55 ms (1.19 PFLOP/s) at 2.05 GHz, matrix
-// units busy in 51% of the cycles and no LDS bank conflicts; on zeros, at 2.4 GHz, 4.55 ms.  12 x 32760 x 512: 128 us (0.81
-// PFLOP/s), a third of it the ends of so short a walk; one query over 12 x 32760 keys: 38 us (5.3 TB/s).  Blocks of four
-// waves, two of them on a CU, overlap these ends but read K and V twice as often: 142 and 148 us with 512 keys, 6.3 ms with
-// 32760.  Walking over several query tiles in one block spills (7.7 ms, and 6.8 with chains of tiles).
+// What bounds it: how much of the softmax and the barriers the other group's matrix work covers, and the chip's power.  12 heads
+// of 32760 x 32760, 128 columns, bf16, take 5.5 ms (1.2 PFLOP/s) at 1.97 GHz, matrix units busy in 58% of the cycles, LDS reading
+// in 29% without bank conflicts; on zeros, at 2.39 GHz, 4.5 ms and 56%.  fp16 6.1 ms.  64 columns 3.64 ms, matrix units busy in
+// 37%, LDS in 28%, 9% bank conflicts of the transposing reads.  12 x 32760 x 512: 130 us (0.8 PFLOP/s), a third of it the ends
+// of so short a walk; one query over 12 x 32760 keys: 38 us (5.3 TB/s).  Blocks of four waves, two of them on a CU, overlap
+// these ends but read K and V twice as often: 142 and 148 us with 512 keys, 6.3 ms with 32760.  Walking over several query
+// tiles in one block spills (7.7 ms, and 6.8 with chains of tiles).
 template <int T, int DP, bool kFull>
 __global__ void __launch_bounds__(kFwdWaves * kWave) __attribute__((amdgpu_waves_per_eu(2, 2)))
 dense_fwd_kernel(DenseArgs a) {

@@ -130,9 +130,10 @@ __device__ __forceinline__ void alternate(int tiles, bool group_b, bool active, 
 
 // dq.  A block: 8 waves of 32 queries, one per lane; K and V tiles of 64 keys double buffered in LDS.  S^T = K Q^T and
 // dP^T = V dO^T leave a query's 16 keys in its lane, and dS^T is at once the operand of dQ^T += K^T dS^T.
-// What bounds it: power.  12 x 32760 x 32760 x 128 takes 8.4 ms (1.18 PFLOP/s of three products) at 2.10 GHz with the matrix
-// units busy in 51% of the cycles; on zeros 7.2.  12 x 32760 x 512: 168 us.  Making
-// delta here in place of its kernel gained 2% of the two there: its loads too come at the blocks' starts.
+// What bounds it: the parts of a step that the other group's matrix work does not cover, and power.  12 x 32760 x 32760 x 128 in
+// bf16 takes 8.2 ms (1.2 PFLOP/s of three products) at 2.03 GHz with the matrix units busy in 56% of the cycles and LDS reading in
+// 28%; on zeros, at 2.39 GHz, 7.2 and 55%.  fp16 8.8, 64 columns 5.5.  12 x 32760 x 512: 168 us.  Making delta here in place of
+// its kernel cost 53 us there where that takes 61, whose loads come at the blocks' starts too: about 3% of the two, not taken.
 template <int T, int DP, bool kFull>
 __global__ void __launch_bounds__(kBwdWaves * kWave) __attribute__((amdgpu_waves_per_eu(2, 2)))
 dense_dq_kernel(DenseArgs a) {
@@ -252,8 +253,9 @@ dense_dq_kernel(DenseArgs a) {
 // S = Q K^T and dP = dO V^T leave a key's 16 queries in its lane; P is at once the operand of dV^T += dO^T P, dS of
 // dK^T += Q^T dS.  The two sums take 128 of a lane's 256 registers and K 32: V's operand is read from LDS where it is used
 // (in registers too, they spill and 11.7 ms become 37).
-// What bounds it: power.  12 x 32760 x 32760 x 128 takes 11.7 ms (1.13 PFLOP/s of four products) at 2.18 GHz with the matrix
-// units busy in 47% of the cycles; on zeros 10.2.  12 x 32760 x 512: 230 us, in shares of the queries.
+// What bounds it: the same.  12 x 32760 x 32760 x 128 in bf16 takes 11.5 ms (1.15 PFLOP/s of four products) at 2.10 GHz with the
+// matrix units busy in 52% of the cycles and LDS reading in 39%; on zeros, at 2.39 GHz, 10.2 and 52%.  fp16 12.5, 64 columns 7.8.
+// 12 x 32760 x 512: 215 us, in shares of the queries.
 template <int T, int DP, bool kFull>
 __global__ void __launch_bounds__(kBwdWaves * kWave) __attribute__((amdgpu_waves_per_eu(2, 2)))
 dense_dkv_kernel(DenseArgs a) {
