@@ -69,6 +69,9 @@ constexpr float kF16PShift = 14.0f;
 // 2^-36 below.  With P = 1 at the maximum, keys 14 bits below it lost bits and those 25 below it were lost, which is all of o
 // where the largest one's value is 0 (even keys at e^-16 and e^-17 of it: o 8% and 44% too large; at e^-18: o = 0).
 constexpr float kF16Top = 12.0f;
+// for maxima below 2^22: a step of those is a quarter at most.  From 2^26 on, with steps of 8, a maximum less 12 may come out 16
+// lower, and P past the type's range.
+constexpr float kF16TopWithin = 4194304.0f;
 
 typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
 

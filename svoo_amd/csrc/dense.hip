@@ -167,7 +167,8 @@ dense_fwd_kernel(DenseArgs a) {
       mx = xhalf_max(mx) * sl;
       // a row's maximum moves for its own sake alone: its bits do not depend on the rows beside it
       const bool moves = xhalf_max(high ? 1.0f : 0.0f) > 0.0f;
-      const float m_new = moves ? fmaxf(m_run, T == kDenseF16 ? mx - kF16Top : mx) : m_run;
+      const float low = T == kDenseF16 && fabsf(mx) < kF16TopWithin ? mx - kF16Top : mx;
+      const float m_new = moves ? fmaxf(m_run, low) : m_run;
       const float alpha = __builtin_amdgcn_exp2f(m_run - m_new);
       m_run = m_new;
       l_run *= alpha;
